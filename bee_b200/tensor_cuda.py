@@ -140,3 +140,99 @@ def rms_norm_rope(x: torch.Tensor, w: torch.Tensor, y: torch.Tensor, seq: int, h
            float(eps), float(theta), pos_offset, _stream(stream))
     _done(sync, stream)
     return y
+
+
+def _current(op: str, *ts) -> None:
+    """Checks that every given tensor lives on the calling thread's current device, where the kernels run."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise BeeError(op, 1, "tensor is not on a CUDA device")
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.device.index != dev:
+            raise BeeError(op, 1, f"tensor is on cuda:{t.device.index}, the current device is cuda:{dev}")
+
+
+def _rows(op: str, name: str, t: torch.Tensor) -> int:
+    """Row stride (in elements) of a 2-D tensor whose rows are contiguous and do not overlap."""
+    if t.dim() != 2:
+        raise BeeError(op, 1, f"{name} must be 2-D")
+    r, c = t.shape
+    s0, s1 = t.stride()
+    if (s1 != 1 and c > 1) or (s0 < c and r > 1):
+        raise BeeError(op, 1, f"{name}: rows must be contiguous and must not overlap")
+    return s0 if r > 1 else max(c, 1)
+
+
+def _vector(op: str, name: str, t, n: int, dtype) -> int:
+    """Pointer of an optional contiguous vector of n elements."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise BeeError(op, 1, f"{name} must be contiguous, {dtype}, with {n} elements")
+    return t.data_ptr()
+
+
+def _targets(op: str, targets, rows: int):
+    if targets is None:
+        return C.I64, None
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise BeeError(op, 1, "targets must be int32 or int64")
+    return DTYPE_CODE[targets.dtype], _vector(op, "targets", targets, rows, targets.dtype)
+
+
+def token_logprobs(logits: torch.Tensor, targets, logprob=None, entropy=None, row_max=None, log_sum=None, *,
+                   temperature: float = 1.0, top_ids=None, top_logprobs=None, stream=None, sync=False):
+    """Log probabilities of `targets` [rows] under softmax(logits / temperature), logits [rows, vocab] (rows may be strided).
+
+    Writes whichever of logprob, entropy, row_max, log_sum (float32 [rows]) and top_ids / top_logprobs (int32 /
+    float32 [rows, k], k <= 32: the k largest logits, equal ones by lowest index) are given.  A negative target means
+    that the row holds no token (logprob 0).  row_max and log_sum are what the backward needs."""
+    op = "token_logprobs"
+    _current(op, logits, targets, logprob, entropy, row_max, log_sum, top_ids, top_logprobs)
+    ld = _rows(op, "logits", logits)
+    rows, vocab = logits.shape
+    f32 = torch.float32
+    if logprob is not None and targets is None:
+        raise BeeError(op, 1, "logprob needs targets")
+    tdt, tptr = _targets(op, targets, rows)
+    if (top_ids is None) != (top_logprobs is None):
+        raise BeeError(op, 1, "top_ids and top_logprobs go together")
+    k = 0
+    if top_ids is not None:
+        if top_ids.dim() != 2 or top_ids.shape[0] != rows:
+            raise BeeError(op, 1, "top_ids must be [rows, k]")
+        k = top_ids.shape[1]
+    C.call("bee_b200_token_logprobs", _code(logits), logits.data_ptr(), ld, tdt, tptr, rows, vocab, float(temperature),
+           _vector(op, "logprob", logprob, rows, f32), _vector(op, "entropy", entropy, rows, f32),
+           _vector(op, "row_max", row_max, rows, f32), _vector(op, "log_sum", log_sum, rows, f32), k,
+           _vector(op, "top_ids", top_ids, rows * k, torch.int32),
+           _vector(op, "top_logprobs", top_logprobs, rows * k, f32), _stream(stream))
+    _done(sync, stream)
+    return logprob
+
+
+def token_logprobs_backward(logits: torch.Tensor, targets, row_max: torch.Tensor, log_sum: torch.Tensor, entropy,
+                            dlogprob, dentropy, dlogits: torch.Tensor, *, temperature: float = 1.0, stream=None,
+                            sync=False):
+    """dlogits = gradient of sum(dlogprob * logprob + dentropy * entropy); row_max, log_sum and entropy come from the
+    forward, dlogprob and dentropy (float32 [rows]) may be None.  dlogits may be logits itself."""
+    op = "token_logprobs_backward"
+    _current(op, logits, targets, row_max, log_sum, entropy, dlogprob, dentropy, dlogits)
+    ld, ldd = _rows(op, "logits", logits), _rows(op, "dlogits", dlogits)
+    rows, vocab = logits.shape
+    f32 = torch.float32
+    if dlogits.dtype != logits.dtype or dlogits.shape != logits.shape:
+        raise BeeError(op, 1, "dlogits must have the logits' dtype and shape")
+    if dlogprob is not None and targets is None:
+        raise BeeError(op, 1, "dlogprob needs targets")
+    tdt, tptr = _targets(op, targets, rows)
+    C.call("bee_b200_token_logprobs_backward", _code(logits), logits.data_ptr(), ld, tdt, tptr, rows, vocab,
+           float(temperature), _vector(op, "row_max", row_max, rows, f32), _vector(op, "log_sum", log_sum, rows, f32),
+           _vector(op, "entropy", entropy, rows, f32), _vector(op, "dlogprob", dlogprob, rows, f32),
+           _vector(op, "dentropy", dentropy, rows, f32), dlogits.data_ptr(), ldd, _stream(stream))
+    _done(sync, stream)
+    return dlogits

@@ -226,6 +226,41 @@ BEE_B200_API int bee_b200_rms_norm_rope(int dt, const void* x, const void* w, vo
                            size_t heads, size_t head_dim, float eps, double theta, size_t pos_offset,
                            bee_b200_stream_t stream);
 
+/* ------------------------------------------------ log probabilities of tokens
+ * New: the reference has no path from logits to probabilities.  Per row of a
+ * [rows, vocab] matrix of logits x (row stride ld >= vocab, in elements), with
+ * m = max x, z_i = (x_i - m) / temperature and S = sum exp(z_i):
+ *   logp_i = z_i - log S,   entropy = log S - sum(exp(z_i) z_i) / S.
+ * dt (the logits) in {F32, BF16, F16}; statistics and outputs are fp32.
+ *   logprob[r]  = logp of targets[r] (I32 or I64); a negative target means "no
+ *                 token here" and gives 0; one >= vocab gives NaN;
+ *   entropy[r], row_max[r] = m, log_sum[r] = log S (the last two are what the
+ *                 backward needs);
+ *   top_ids, top_logprobs [rows, top]: the `top` (<= 32, <= vocab) largest
+ *                 logits in descending order, equal ones by lowest index.
+ * logprob (with targets), entropy, row_max and log_sum may each be NULL, and
+ * top 0.  Logits of -inf (masked) have probability 0; a row of nothing else
+ * gives logprob, row_max, log_sum and top_logprobs -inf and entropy 0.  A row that
+ * holds a NaN or +inf gives NaN (top_ids -1; row_max its largest number).  Logits need only the alignment
+ * of their type.  One pass, no workspace; few rows are shared by clusters of CTAs. */
+BEE_B200_API int bee_b200_token_logprobs(int dt, const void* logits, size_t ld, int targets_dt, const void* targets,
+                                         size_t rows, size_t vocab, float temperature, float* logprob, float* entropy,
+                                         float* row_max, float* log_sum, size_t top, int32_t* top_ids,
+                                         float* top_logprobs, bee_b200_stream_t stream);
+
+/* Gradient of sum(dlogprob logprob + dentropy entropy) with respect to the logits:
+ *   dlogits_i = (dlogprob (delta_{i,target} - p_i) - dentropy p_i (logp_i + entropy)) / temperature
+ * in the logits' dtype (row stride ldd).  row_max, log_sum and (when dentropy is
+ * given) entropy are the forward's outputs; dlogprob (with targets) and dentropy
+ * may each be NULL.  Rows without a token take no gradient from dlogprob; rows
+ * whose gradients are both 0, and rows with every logit masked, get zeros
+ * whatever they hold.  dlogits may be the logits themselves (same stride). */
+BEE_B200_API int bee_b200_token_logprobs_backward(int dt, const void* logits, size_t ld, int targets_dt,
+                                                  const void* targets, size_t rows, size_t vocab, float temperature,
+                                                  const float* row_max, const float* log_sum, const float* entropy,
+                                                  const float* dlogprob, const float* dentropy, void* dlogits,
+                                                  size_t ldd, bee_b200_stream_t stream);
+
 /* ------------------------------------------------------------------ matmul */
 
 /* C[M,N] = A[M,K] . B[K,N], row-major contiguous, same dtype.

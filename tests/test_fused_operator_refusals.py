@@ -1,0 +1,58 @@
+"""Calls that the fused operators refuse, on the host: no kernel is launched."""
+import math
+
+import pytest
+
+from bee_b200 import _capi
+
+P = 4096  # a 16-byte aligned address that is never read: every call here is refused first
+F32, BF16, F16, I32, I64 = _capi.F32, _capi.BF16, _capi.F16, _capi.I32, _capi.I64
+
+
+def refused(name, *args):
+    rc = getattr(_capi.lib(), name)(*args)
+    msg = _capi.last_error()
+    assert rc == 1 and msg, (name, rc, msg)
+    return msg
+
+
+def accepted(name, *args):
+    assert getattr(_capi.lib(), name)(*args) == 0, _capi.last_error()
+
+
+def logprobs(dt=BF16, logits=P, ld=64, tdt=I64, targets=P, rows=4, vocab=64, temperature=1.0, logprob=P, entropy=P,
+             row_max=P, log_sum=P, top=0, ids=None, lps=None):
+    return ("bee_b200_token_logprobs", dt, logits, ld, tdt, targets, rows, vocab, temperature, logprob, entropy, row_max,
+            log_sum, top, ids, lps, None)
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"dt": I32}, "dtype"), ({"logits": None}, "null"), ({"ld": 63}, "stride"), ({"tdt": F32}, "targets"),
+    ({"targets": None}, "null"), ({"vocab": 0, "ld": 0}, "vocab"), ({"vocab": 2 ** 31, "ld": 2 ** 31}, "vocab"),
+    ({"temperature": 0.0}, "temperature"), ({"temperature": -1.0}, "temperature"), ({"temperature": math.nan}, "temperature"),
+    ({"temperature": math.inf}, "temperature"), ({"temperature": 1e-45}, "temperature"), ({"top": 33, "ids": P, "lps": P}, "alternatives"),
+    ({"top": 9, "vocab": 8, "ids": P, "lps": P}, "alternatives"), ({"top": 2, "lps": P}, "null"), ({"top": 2, "ids": P}, "null"),
+    ({"logits": P + 1}, "aligned"), ({"dt": F32, "logits": P + 2}, "aligned"),
+])
+def test_logprobs_refusals(change, word):
+    assert word in refused(*logprobs(**change))
+
+
+def test_logprobs_of_no_rows():
+    accepted(*logprobs(rows=0, logits=None, targets=None, logprob=None, entropy=None, row_max=None, log_sum=None))
+
+
+def logprobs_backward(dt=BF16, logits=P, ld=64, tdt=I64, targets=P, rows=4, vocab=64, temperature=1.0, row_max=P, log_sum=P,
+                      entropy=P, dlogprob=P, dentropy=P, dlogits=2 * P, ldd=64):
+    return ("bee_b200_token_logprobs_backward", dt, logits, ld, tdt, targets, rows, vocab, temperature, row_max, log_sum,
+            entropy, dlogprob, dentropy, dlogits, ldd, None)
+
+
+@pytest.mark.parametrize("change,word", [
+    ({"dt": I64}, "dtype"), ({"logits": None}, "null"), ({"dlogits": None}, "null"), ({"ld": 63}, "stride"), ({"ldd": 10}, "stride"),
+    ({"row_max": None}, "null"), ({"log_sum": None}, "null"), ({"entropy": None}, "null"), ({"targets": None}, "null"),
+    ({"tdt": BF16}, "targets"), ({"temperature": 0.0}, "temperature"), ({"dlogits": P, "ldd": 72}, "in place"),
+    ({"dlogits": 2 * P + 1}, "aligned"), ({"vocab": 0}, "vocab"),
+])
+def test_logprobs_backward_refusals(change, word):
+    assert word in refused(*logprobs_backward(**change))
