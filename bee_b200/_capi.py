@@ -65,6 +65,9 @@ SIGNATURES = {
     "bee_b200_rms_norm_rows": [_i, _vp, _vp, _vp, _sz, _sz, _f, _vp],
     "bee_b200_rope": [_i, _vp, _vp, _sz, _sz, _sz, _sz, _d, _sz, _vp],
     "bee_b200_rms_norm_rope": [_i, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _f, _d, _sz, _vp],
+    "bee_b200_norm_gate_residual": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _f, _f, _f, _vp],
+    "bee_b200_norm_gate_residual_backward": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz,
+                                             _sz, _f, _f, _f, _vp],
     "bee_b200_token_logprobs": [_i, _vp, _sz, _i, _vp, _sz, _sz, _f, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp],
     "bee_b200_token_logprobs_backward": [_i, _vp, _sz, _i, _vp, _sz, _sz, _f, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     "bee_b200_matmul": [_i, _vp, _vp, _vp, _sz, _sz, _sz, _vp],

@@ -1,0 +1,685 @@
+// The step from one block's output to the next block's input, in one pass, and
+// its gradient:
+//   n  = h rstd(h) w_post            (n = h without w_post)
+//   x' = alpha x + beta gate n       (gate: one row, or one row per group of rows)
+//   y  = x' rstd(x') w_pre
+// with rstd(v) = 1 / sqrt(mean(v^2) + eps) over a row.  New: the reference has
+// no normalisation; rms_norm_rows is the unfused form.
+//
+// Backward, from the forward's inputs and the gradients dx', dy of its outputs
+// (statistics and x' are recomputed, nothing has to be kept):
+//   xh = x' rstd(x'),  D = dx' + rstd(x') (dy w_pre - xh mean(dy w_pre xh))
+//   dx = alpha D,      dn = beta gate D,      hh = h rstd(h)
+//   dh = rstd(h) (dn w_post - hh mean(dn w_post hh))
+//   dw_pre = sum_rows dy xh,  dw_post = sum_rows dn hh,  dgate = sum_group beta D n
+//
+// Both are bound by HBM (forward: 2 reads and 2 writes of the tensor, backward:
+// 4 and 2).  A CTA owns whole rows, so every tensor crosses HBM once: upcoming
+// rows are copied into a shared-memory ring with cp.async while the current one
+// is reduced (1 or 2 block reductions forward, 3 backward).  All arithmetic is
+// fp32, in packed pairs; results are rounded once, when stored.
+//
+// A thread owns the same kEpt = 16 columns of every row, so the backward's three
+// column sums stay in registers over the CTA's contiguous range of rows; each CTA
+// writes one row of partial sums and a second kernel adds them in a fixed order
+// (results do not depend on timing).  A group of rows that lies inside one
+// CTA's range is finished there; one that is cut leaves a partial per CTA.
+//
+// Rows of any length up to 16384 (fp32: 12288): if it is a whole number of 16-byte vectors and
+// all tensors are 16-byte aligned, each thread copies and reads only its own
+// vectors (no barrier for the ring); otherwise the block copies the aligned
+// 16-byte blocks that cover the row and threads read single elements from them.
+#include <cmath>
+#include <type_traits>
+
+#include "common.cuh"
+#include "sm100.cuh"
+
+namespace bee_b200 {
+
+namespace {
+
+constexpr int kEpt = 16;         // columns per thread
+constexpr int kPairs = kEpt / 2;
+// 1024 threads' columns; in fp32, what the four rows of a backward slot leave in shared memory
+constexpr size_t max_cols(int dt) { return dt == DT_F32 ? 12288 : 16384; }
+using f2 = uint64_t;             // two fp32 values
+
+__device__ __forceinline__ f2 dup(float v) { return pack_f32x2(v, v); }
+__device__ __forceinline__ float hsum(f2 v) {
+    float a, b;
+    unpack_f32x2(v, a, b);
+    return a + b;
+}
+
+template <typename T> struct Conv;
+template <> struct Conv<float> {
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct Conv<__nv_bfloat16> {
+    static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ f2 up2(uint32_t w) { return bf16x2_to_f32x2(w); }
+    static __device__ __forceinline__ uint32_t down2(f2 v) { return f32x2_to_bf16x2(v); }
+};
+template <> struct Conv<__half> {
+    static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ f2 up2(uint32_t w) {
+        const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w));
+        return pack_f32x2(f.x, f.y);
+    }
+    static __device__ __forceinline__ uint32_t down2(f2 v) {
+        float a, b;
+        unpack_f32x2(v, a, b);
+        return pack_f16x2(a, b);
+    }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_wait(int pending) {
+    if (pending == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+}
+
+// The columns of one thread.  VEC: 16-byte vectors tid, tid + THREADS, ...;
+// otherwise columns tid, tid + THREADS, ....  Columns past the row read as 0
+// and are not written, so they add nothing to any sum.
+template <typename T, bool VEC, int THREADS> struct Cols {
+    static constexpr int E = 16 / sizeof(T);
+    uint32_t cols;
+    __device__ __forceinline__ explicit Cols(uint32_t n) : cols(n) {}
+    __device__ __forceinline__ static uint32_t vec(int j) { return j * THREADS + threadIdx.x; }
+    __device__ __forceinline__ static uint32_t col(int k) { return k * THREADS + threadIdx.x; }
+
+    static __device__ __forceinline__ void unpack(uint4 q, f2* v) {
+        if constexpr (std::is_same_v<T, float>) {
+            v[0] = pack_f32x2(__uint_as_float(q.x), __uint_as_float(q.y));
+            v[1] = pack_f32x2(__uint_as_float(q.z), __uint_as_float(q.w));
+        } else {
+            v[0] = Conv<T>::up2(q.x); v[1] = Conv<T>::up2(q.y); v[2] = Conv<T>::up2(q.z); v[3] = Conv<T>::up2(q.w);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const f2* v) {
+        if constexpr (std::is_same_v<T, float>) {
+            float a, b, c, d;
+            unpack_f32x2(v[0], a, b);
+            unpack_f32x2(v[1], c, d);
+            return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c), __float_as_uint(d));
+        } else {
+            return make_uint4(Conv<T>::down2(v[0]), Conv<T>::down2(v[1]), Conv<T>::down2(v[2]), Conv<T>::down2(v[3]));
+        }
+    }
+    // from a row (shared or global memory; LDG: read-only global vectors)
+    template <bool LDG> __device__ __forceinline__ void read(const T* p, f2 (&v)[kPairs]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int j = 0; j < kEpt / E; ++j) {
+                const uint4* q = reinterpret_cast<const uint4*>(p) + vec(j);
+                unpack(vec(j) * E < cols ? (LDG ? __ldg(q) : *q) : make_uint4(0, 0, 0, 0), v + j * (E / 2));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k)
+                v[k] = pack_f32x2(col(2 * k) < cols ? Conv<T>::up(p[col(2 * k)]) : 0.f,
+                                  col(2 * k + 1) < cols ? Conv<T>::up(p[col(2 * k + 1)]) : 0.f);
+        }
+    }
+    // an optional vector of weights; absent: ones
+    __device__ __forceinline__ void weights(const T* p, f2 (&v)[kPairs]) const {
+        if (p) {
+            read<true>(p, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = dup(1.f);
+        }
+    }
+    __device__ __forceinline__ void write(T* p, const f2 (&v)[kPairs]) const {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int j = 0; j < kEpt / E; ++j)
+                if (vec(j) * E < cols) __stcs(reinterpret_cast<uint4*>(p) + vec(j), pack(v + j * (E / 2)));
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                float a, b;
+                unpack_f32x2(v[k], a, b);
+                if (col(2 * k) < cols) p[col(2 * k)] = Conv<T>::down(a);
+                if (col(2 * k + 1) < cols) p[col(2 * k + 1)] = Conv<T>::down(b);
+            }
+        }
+    }
+    // fp32 partial sums, in this thread's own order (any fixed place per column would do)
+    __device__ __forceinline__ void write_f32(float* p, const f2 (&v)[kPairs]) const {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            float a, b;
+            unpack_f32x2(v[k], a, b);
+            const uint32_t ca = VEC ? vec(2 * k / E) * E + 2 * k % E : col(2 * k);
+            const uint32_t cb = VEC ? ca + 1 : col(2 * k + 1);
+            if (ca < cols) p[ca] = a;
+            if (cb < cols) p[cb] = b;
+        }
+    }
+    __device__ __forceinline__ void read_f32(const float* p, f2 (&v)[kPairs]) const {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            const uint32_t ca = VEC ? vec(2 * k / E) * E + 2 * k % E : col(2 * k);
+            const uint32_t cb = VEC ? ca + 1 : col(2 * k + 1);
+            v[k] = pack_f32x2(ca < cols ? p[ca] : 0.f, cb < cols ? p[cb] : 0.f);
+        }
+    }
+};
+
+// Sums over the block with one barrier: consecutive calls use alternating halves
+// of `red`, so a call's writes never meet the previous call's reads.
+template <int THREADS> struct BlockSum {
+    float2 (*red)[THREADS / 32];
+    int parity = 0;
+    __device__ __forceinline__ float2 operator()(float a, float b) {
+        a = warp_sum(a);
+        b = warp_sum(b);
+        if constexpr (THREADS == 32) return make_float2(a, b);
+        if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = make_float2(a, b);
+        __syncthreads();
+        float2 r = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            const float2 v = red[parity][w];
+            r.x += v.x;
+            r.y += v.y;
+        }
+        parity ^= 1;
+        return r;
+    }
+};
+
+// A ring of `stages` slots, each one row of up to NT tensors.
+template <typename T, bool VEC, int THREADS, int NT> struct Ring {
+    const T* src[NT];
+    uint8_t* base;
+    uint32_t cols, pitch, stages;  // pitch: bytes of one tensor's row in a slot
+    long long row, end;            // next row to copy
+    uint32_t slot = 0;             // its slot
+
+    __device__ __forceinline__ uint8_t* at(uint32_t s, int t) const { return base + (s * NT + t) * pitch; }
+    // bytes of tensor t's row r that precede it in its slot
+    __device__ __forceinline__ uint32_t lead(int t, long long r) const {
+        return VEC ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(src[t] + r * cols) & 15u);
+    }
+    __device__ __forceinline__ const T* read(uint32_t s, int t, long long r) const {
+        return reinterpret_cast<const T*>(at(s, t) + lead(t, r));
+    }
+    __device__ __forceinline__ void issue() {
+        if (row < end) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (!src[t]) continue;
+                const T* g = src[t] + row * cols;
+                if constexpr (VEC) {
+                    constexpr uint32_t E = 16 / sizeof(T);
+                    const uint32_t dst = sm100::smem_u32(at(slot, t));
+#pragma unroll
+                    for (int j = 0; j < kEpt / static_cast<int>(E); ++j) {
+                        const uint32_t v = j * THREADS + threadIdx.x;
+                        if (v * E < cols) cp_async16(dst + v * 16, reinterpret_cast<const uint4*>(g) + v, 16);
+                    }
+                } else {
+                    // the 16-byte blocks that cover the row; the last is cut at the row's end, and one
+                    // that begins before the tensor is copied element by element
+                    const uint32_t ld = lead(t, row), bytes = ld + cols * static_cast<uint32_t>(sizeof(T));
+                    const uint8_t* a = reinterpret_cast<const uint8_t*>(g) - ld;
+                    for (uint32_t o = threadIdx.x * 16; o < bytes; o += THREADS * 16) {
+                        if (o == 0 && row == 0 && ld != 0) {
+                            for (uint32_t b = ld; b < 16 && b < bytes; b += sizeof(T))
+                                *reinterpret_cast<T*>(at(slot, t) + b) = *reinterpret_cast<const T*>(a + b);
+                        } else {
+                            cp_async16(sm100::smem_u32(at(slot, t) + o), a + o, bytes - o < 16 ? bytes - o : 16);
+                        }
+                    }
+                }
+            }
+        }
+        cp_commit();  // one group per row, empty past the end, so that the wait counts stay uniform
+        ++row;
+        slot = slot + 1 == stages ? 0 : slot + 1;
+    }
+    // Waits for the current row's copies and starts those of a later row in the slot that is free by then.
+    __device__ __forceinline__ void advance() {
+        if (stages == 1) {
+            if constexpr (!VEC) __syncthreads();
+            issue();
+            cp_wait(0);
+            if constexpr (!VEC) __syncthreads();
+        } else {
+            cp_wait(static_cast<int>(stages) - 2);
+            if constexpr (!VEC) __syncthreads();  // the row is complete, and its predecessor's slot has been read by all
+            issue();
+        }
+    }
+    __device__ __forceinline__ void start() {
+        for (uint32_t s = 1; s < stages; ++s) issue();
+    }
+};
+
+struct NormArgs {
+    const void *h, *x, *w_post, *gate, *w_pre;
+    void *x_out, *y;
+    const void *dx_out, *dy;
+    void *dh, *dx, *dgate;
+    float *part_post, *part_pre, *part_gate;  // partial sums: [ctas][cols], [ctas][cols], [2 * ctas][cols]
+    long long rows, per_cta, group;           // group: rows per gate row
+    uint32_t cols, pitch, stages;
+    float alpha, beta, eps;
+};
+
+// ---------------------------------------------------------------- forward
+
+template <typename T, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(const NormArgs a) {
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ float2 red[2][THREADS / 32];
+    BlockSum<THREADS> block_sum{red};
+    const Cols<T, VEC, THREADS> cl(a.cols);
+    const long long r0 = blockIdx.x * a.per_cta;
+    const long long r1 = r0 + a.per_cta < a.rows ? r0 + a.per_cta : a.rows;
+    const T *wpost = static_cast<const T*>(a.w_post), *wpre = static_cast<const T*>(a.w_pre);
+    const float inv_n = 1.0f / static_cast<float>(a.cols);
+    Ring<T, VEC, THREADS, 2> ring{{static_cast<const T*>(a.h), static_cast<const T*>(a.x)}, ring_smem, a.cols, a.pitch, a.stages, r0, r1};
+    pdl_wait();
+    ring.start();
+    uint32_t slot = 0;
+    for (long long r = r0; r < r1; ++r, slot = slot + 1 == a.stages ? 0 : slot + 1) {
+        if (r + 1 >= r1) pdl_trigger();
+        ring.advance();
+        f2 v[kPairs], t[kPairs];
+        cl.template read<false>(ring.read(slot, 0, r), v);
+        float scale = a.beta;
+        if (wpost) {
+            f2 ss = 0;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(v[k], v[k], ss);
+            scale *= rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps));
+            cl.weights(wpost, t);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], t[k]);
+        }
+        if (a.gate) {
+            cl.weights(static_cast<const T*>(a.gate) + (r / a.group) * a.cols, t);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], t[k]);
+        }
+        cl.template read<false>(ring.read(slot, 1, r), t);
+        f2 ss = 0;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            v[k] = fma_f32x2(v[k], dup(scale), mul_f32x2(t[k], dup(a.alpha)));
+            ss = fma_f32x2(v[k], v[k], ss);
+        }
+        cl.write(static_cast<T*>(a.x_out) + r * a.cols, v);
+        if (wpre) {
+            const f2 rx = dup(rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps)));
+            cl.weights(wpre, t);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(mul_f32x2(v[k], rx), t[k]);
+            cl.write(static_cast<T*>(a.y) + r * a.cols, v);
+        }
+    }
+    cp_wait(0);
+}
+
+// ---------------------------------------------------------------- backward
+
+// REG: the column sums stay in registers; otherwise (rows too wide for that) in
+// the CTA's own rows of the partial sums, read and written once per row.
+template <typename T, bool VEC, int THREADS, bool REG>
+__global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    __shared__ float2 red[2][THREADS / 32];
+    BlockSum<THREADS> block_sum{red};
+    const Cols<T, VEC, THREADS> cl(a.cols);
+    const long long r0 = blockIdx.x * a.per_cta;
+    const long long r1 = r0 + a.per_cta < a.rows ? r0 + a.per_cta : a.rows;
+    const T *wpost = static_cast<const T*>(a.w_post), *wpre = static_cast<const T*>(a.w_pre);
+    const T* gate = static_cast<const T*>(a.gate);
+    const float inv_n = 1.0f / static_cast<float>(a.cols);
+    Ring<T, VEC, THREADS, 4> ring{{static_cast<const T*>(a.h), static_cast<const T*>(a.x), static_cast<const T*>(a.dx_out),
+                                   static_cast<const T*>(a.dy)}, ring_smem, a.cols, a.pitch, a.stages, r0, r1};
+    float* my_post = a.part_post + static_cast<long long>(blockIdx.x) * a.cols;
+    float* my_pre = a.part_pre + static_cast<long long>(blockIdx.x) * a.cols;
+    float* my_gate = a.part_gate + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+    f2 s_post[kPairs], s_pre[kPairs], s_gate[kPairs];
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) s_post[k] = s_pre[k] = s_gate[k] = 0;
+    pdl_wait();
+    ring.start();
+    long long group = gate ? r0 / a.group : 0;
+    long long group_end = gate ? (group + 1) * a.group : r1;
+    bool first_of_group = true, first = true;
+    uint32_t slot = 0;
+    for (long long r = r0; r < r1; ++r, slot = slot + 1 == a.stages ? 0 : slot + 1) {
+        ring.advance();
+        const T* gate_row = gate ? gate + group * a.cols : nullptr;
+        f2 hh[kPairs], v[kPairs], w[kPairs], t[kPairs];
+        // hh = h rstd(h), v = x'
+        cl.template read<false>(ring.read(slot, 0, r), hh);
+        float rh = 1.f;
+        if (wpost) {
+            f2 ss = 0;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(hh[k], hh[k], ss);
+            rh = rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps));
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) hh[k] = mul_f32x2(hh[k], dup(rh));
+        }
+        cl.weights(wpost, w);
+        cl.weights(gate_row, t);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(mul_f32x2(hh[k], w[k]), mul_f32x2(t[k], dup(a.beta)));
+        cl.template read<false>(ring.read(slot, 1, r), t);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) v[k] = fma_f32x2(t[k], dup(a.alpha), v[k]);
+        // v = D
+        if (wpre) {
+            cl.template read<false>(ring.read(slot, 3, r), t);
+            cl.weights(wpre, w);
+            f2 ss = 0, dot = 0;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                ss = fma_f32x2(v[k], v[k], ss);
+                dot = fma_f32x2(mul_f32x2(t[k], w[k]), v[k], dot);
+            }
+            const float2 sum = block_sum(hsum(ss), hsum(dot));
+            const float rx = rsqrtf(fmaf(sum.x, inv_n, a.eps));
+            const f2 rx2 = dup(rx), mean = dup(-rx * sum.y * inv_n);  // -mean(dy w_pre xh)
+            if constexpr (!REG) if (!first) cl.read_f32(my_pre, s_pre);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                const f2 xh = mul_f32x2(v[k], rx2);
+                s_pre[k] = fma_f32x2(t[k], xh, s_pre[k]);
+                v[k] = mul_f32x2(fma_f32x2(xh, mean, mul_f32x2(t[k], w[k])), rx2);
+            }
+            if constexpr (!REG) cl.write_f32(my_pre, s_pre);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = 0;
+        }
+        if (a.dx_out) {
+            cl.template read<false>(ring.read(slot, 2, r), t);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = add_f32x2(v[k], t[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) t[k] = mul_f32x2(v[k], dup(a.alpha));
+        cl.write(static_cast<T*>(a.dx) + r * a.cols, t);
+        // dn = beta gate D and its sums
+        cl.weights(wpost, w);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], dup(a.beta));
+        if (gate) {
+            if constexpr (!REG) {
+                if (!first_of_group) cl.read_f32(my_gate + a.cols, s_gate);
+                else {
+#pragma unroll
+                    for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
+                }
+            }
+            cl.weights(gate_row, t);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                s_gate[k] = fma_f32x2(v[k], mul_f32x2(hh[k], w[k]), s_gate[k]);
+                v[k] = mul_f32x2(v[k], t[k]);
+            }
+            if constexpr (!REG) cl.write_f32(my_gate + a.cols, s_gate);
+        }
+        if (wpost) {
+            if constexpr (!REG) if (!first) cl.read_f32(my_post, s_post);
+            f2 dot = 0;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                s_post[k] = fma_f32x2(v[k], hh[k], s_post[k]);
+                v[k] = mul_f32x2(v[k], w[k]);
+                dot = fma_f32x2(v[k], hh[k], dot);
+            }
+            if constexpr (!REG) cl.write_f32(my_post, s_post);
+            const f2 mean = dup(-block_sum(hsum(dot), 0.f).x * inv_n);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(fma_f32x2(hh[k], mean, v[k]), dup(rh));
+        }
+        cl.write(static_cast<T*>(a.dh) + r * a.cols, v);
+        first = first_of_group = false;
+        // the group ends here: finished if it began in this range, else a partial sum
+        if (gate && (r + 1 == group_end || r + 1 == r1)) {
+            const long long begin = group * a.group;
+            if (begin >= r0 && group_end <= r1) cl.write(static_cast<T*>(a.dgate) + group * a.cols, s_gate);
+            else cl.write_f32(my_gate + (begin < r0 ? 0 : a.cols), s_gate);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
+            first_of_group = true;
+            ++group;
+            group_end += a.group;
+        }
+    }
+    pdl_trigger();
+    if constexpr (REG) {
+        if (wpost) cl.write_f32(my_post, s_post);
+        if (wpre) cl.write_f32(my_pre, s_pre);
+    }
+    cp_wait(0);
+}
+
+// Adds the CTAs' partial sums.  Item 0 is w_post, 1 is w_pre, 1 + c (0 < c < ctas)
+// the gate group that the border between CTAs c - 1 and c is the first to cut, if
+// there is one.  A block takes 32 columns; its 8 warps add every 8th CTA's row and
+// join them in order.
+struct SumArgs {
+    const float *part_post, *part_pre, *part_gate;
+    void *dw_post, *dw_pre, *dgate;
+    long long per_cta, group;
+    uint32_t cols;
+    int ctas;
+};
+
+template <typename T> __global__ void __launch_bounds__(256) norm_residual_sum_kernel(const SumArgs a) {
+    __shared__ float part[8][33];
+    const int cx = threadIdx.x & 31, seg = threadIdx.x >> 5;
+    const uint32_t col = blockIdx.x * 32 + cx;
+    pdl_wait();
+    const int items = a.dgate ? a.ctas + 1 : 2;
+    for (int item = blockIdx.y; item < items; item += gridDim.y) {
+        const float* src;
+        T* dst;
+        long long c0 = 0, c1 = a.ctas, stride = a.cols, begin = 0;
+        if (item < 2) {
+            src = item == 0 ? a.part_post : a.part_pre;
+            dst = static_cast<T*>(item == 0 ? a.dw_post : a.dw_pre);
+            if (!dst) continue;
+        } else {
+            const long long border = static_cast<long long>(item - 1) * a.per_cta, g = border / a.group;
+            begin = g * a.group;
+            if (begin == border || begin < border - a.per_cta) continue;  // not cut here, or cut before
+            c0 = item - 2;
+            c1 = (begin + a.group - 1) / a.per_cta + 1;
+            src = a.part_gate;
+            dst = static_cast<T*>(a.dgate) + g * a.cols;
+            stride = 2 * static_cast<long long>(a.cols);
+        }
+        float s = 0.f;
+        if (col < a.cols)
+            for (long long c = c0 + seg; c < c1; c += 8) {
+                // a CTA keeps the group that it begins inside of in its first slot, one that begins in it in its second
+                const uint32_t second = item >= 2 && c * a.per_cta <= begin ? a.cols : 0;
+                s += src[c * stride + second + col];
+            }
+        part[seg][cx] = s;
+        __syncthreads();
+        if (seg == 0 && col < a.cols) {
+#pragma unroll
+            for (int w = 1; w < 8; ++w) s += part[w][cx];
+            dst[col] = Conv<T>::down(s);
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+constexpr int kRingBytes = 200 * 1024;  // shared memory of one SM given to rings
+
+// Ring of a CTA when `per_sm` of them share an SM: up to 3 rows.
+void plan_ring(NormArgs& a, size_t elem, int tensors, int per_sm, bool vec) {
+    a.pitch = static_cast<uint32_t>((a.cols * elem + 15) / 16 * 16 + (vec ? 0 : 16));
+    const uint32_t slot = a.pitch * static_cast<uint32_t>(tensors);
+    const uint32_t fit = static_cast<uint32_t>(kRingBytes / per_sm) / slot;
+    a.stages = fit < 1 ? 1 : fit > 3 ? 3 : fit;
+}
+
+template <typename T, bool VEC, int THREADS> int launch_fwd(NormArgs a, cudaStream_t st) {
+    constexpr int per_sm = THREADS == 32 ? 24 : 1024 / THREADS;
+    plan_ring(a, sizeof(T), 2, per_sm, VEC);
+    auto norm_kern = norm_residual_kernel<T, VEC, THREADS>;
+    const int smem = static_cast<int>(a.pitch * 2 * a.stages);
+    static SmemLimit limit;
+    if (int rc = limit.ensure(norm_kern, smem, "norm_gate_residual")) return rc;
+    const long long cap = static_cast<long long>(sm_count()) * per_sm;
+    a.per_cta = (a.rows + cap - 1) / cap;
+    launch_pdl(norm_kern, static_cast<unsigned>((a.rows + a.per_cta - 1) / a.per_cta), THREADS, static_cast<size_t>(smem), st, a);
+    return launch_status("norm_gate_residual");
+}
+
+template <typename T, bool VEC> int forward(const NormArgs& a, cudaStream_t st) {
+    if (a.cols <= 32 * kEpt) return launch_fwd<T, VEC, 32>(a, st);
+    if (a.cols <= 128 * kEpt) return launch_fwd<T, VEC, 128>(a, st);
+    if (a.cols <= 256 * kEpt) return launch_fwd<T, VEC, 256>(a, st);
+    if (a.cols <= 512 * kEpt) return launch_fwd<T, VEC, 512>(a, st);
+    return launch_fwd<T, VEC, 1024>(a, st);
+}
+
+struct NormGrads {
+    void *dw_post, *dgate, *dw_pre;
+};
+
+template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const NormGrads& g, cudaStream_t st) {
+    constexpr int per_sm = THREADS == 32 ? 16 : THREADS <= 512 ? 512 / THREADS : 1;
+    plan_ring(a, sizeof(T), 4, per_sm, VEC);
+    auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS, (THREADS < 1024)>;
+    const int smem = static_cast<int>(a.pitch * 4 * a.stages);
+    static SmemLimit limit;
+    if (int rc = limit.ensure(norm_grad_kern, smem, "norm_gate_residual_backward")) return rc;
+    const long long cap = static_cast<long long>(sm_count()) * per_sm;
+    a.per_cta = (a.rows + cap - 1) / cap;
+    const long long ctas = (a.rows + a.per_cta - 1) / a.per_cta;
+    const size_t bytes = static_cast<size_t>(a.cols) * static_cast<size_t>(ctas) * 4 * sizeof(float);
+    void* mem = nullptr;
+    cudaError_t e = pool_malloc(&mem, bytes, st);
+    if (e != cudaSuccess) return api_fail(e, "norm_gate_residual_backward: scratch of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    a.part_post = static_cast<float*>(mem);
+    a.part_pre = a.part_post + static_cast<size_t>(ctas) * a.cols;
+    a.part_gate = a.part_pre + static_cast<size_t>(ctas) * a.cols;
+    launch_pdl(norm_grad_kern, static_cast<unsigned>(ctas), THREADS, static_cast<size_t>(smem), st, a);
+    int rc = launch_status("norm_gate_residual_backward");
+    if (rc == 0) {
+        const SumArgs s{a.part_post, a.part_pre, a.part_gate, g.dw_post, g.dw_pre, g.dgate, a.per_cta, a.group, a.cols,
+                        static_cast<int>(ctas)};
+        const long long items = g.dgate ? ctas + 1 : 2;
+        const dim3 grid((a.cols + 31) / 32, static_cast<unsigned>(items < 64 ? items : 64));
+        launch_pdl(norm_residual_sum_kernel<T>, grid, 256, 0, st, s);
+        rc = launch_status("norm_gate_residual_backward (sums)");
+    }
+    const cudaError_t e2 = cudaFreeAsync(mem, st);
+    if (rc == 0 && e2 != cudaSuccess) rc = api_fail(e2, "norm_gate_residual_backward: %s", cudaGetErrorString(e2));
+    return rc;
+}
+
+template <typename T, bool VEC> int backward(const NormArgs& a, const NormGrads& g, cudaStream_t st) {
+    if (a.cols <= 32 * kEpt) return launch_bwd<T, VEC, 32>(a, g, st);
+    if (a.cols <= 128 * kEpt) return launch_bwd<T, VEC, 128>(a, g, st);
+    if (a.cols <= 256 * kEpt) return launch_bwd<T, VEC, 256>(a, g, st);
+    if (a.cols <= 512 * kEpt) return launch_bwd<T, VEC, 512>(a, g, st);
+    return launch_bwd<T, VEC, 1024>(a, g, st);
+}
+
+int check(const char* what, int dt, size_t rows, size_t cols, size_t group, bool gate, float alpha, float beta, float eps) {
+    if (dt != DT_F32 && dt != DT_BF16 && dt != DT_F16) return fail(cudaErrorInvalidValue, "%s: unsupported dtype %d", what, dt);
+    if (cols == 0 || cols > max_cols(dt)) return fail(cudaErrorInvalidValue, "%s: %zu columns outside [1, %zu]", what, cols, max_cols(dt));
+    if (rows > (size_t{1} << 40)) return fail(cudaErrorInvalidValue, "%s: %zu rows", what, rows);
+    if (gate && group != 0 && rows % group != 0)
+        return fail(cudaErrorInvalidValue, "%s: %zu rows are not a multiple of the gate's group of %zu", what, rows, group);
+    if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(cudaErrorInvalidValue, "%s: eps must be finite and >= 0", what);
+    if (!std::isfinite(alpha) || !std::isfinite(beta)) return fail(cudaErrorInvalidValue, "%s: alpha and beta must be finite", what);
+    return 0;
+}
+
+// Every given pointer is aligned to `to` bytes.
+template <typename... P> bool aligned(uintptr_t to, const P*... p) { return (((reinterpret_cast<uintptr_t>(p)) | ...) & (to - 1)) == 0; }
+
+}  // namespace
+
+}  // namespace bee_b200
+
+using namespace bee_b200;
+
+extern "C" {
+
+int bee_b200_norm_gate_residual(int dt, const void* h, const void* x, const void* w_post, const void* gate, const void* w_pre,
+                                void* x_out, void* y, size_t rows, size_t cols, size_t group, float alpha, float beta,
+                                float eps, bee_b200_stream_t stream) {
+    const char* what = "norm_gate_residual";
+    if (int rc = check(what, dt, rows, cols, group, gate != nullptr, alpha, beta, eps)) return rc;
+    if (rows == 0) return ok();
+    if (!h || !x || !x_out || (w_pre && !y)) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
+    const size_t elem = dt == DT_F32 ? 4 : 2;
+    if (!aligned(elem, h, x, w_post, gate, w_pre, x_out, y))
+        return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    NormArgs a{};
+    a.h = h; a.x = x; a.w_post = w_post; a.gate = gate; a.w_pre = w_pre; a.x_out = x_out; a.y = y;
+    a.rows = static_cast<long long>(rows);
+    a.group = static_cast<long long>(group ? group : rows);
+    a.cols = static_cast<uint32_t>(cols);
+    a.alpha = alpha; a.beta = beta; a.eps = eps;
+    const bool vec = cols * elem % 16 == 0 && aligned(16, h, x, w_post, gate, w_pre, x_out, y);
+    cudaStream_t st = as_stream(stream);
+    if (dt == DT_F32) return vec ? forward<float, true>(a, st) : forward<float, false>(a, st);
+    if (dt == DT_BF16) return vec ? forward<__nv_bfloat16, true>(a, st) : forward<__nv_bfloat16, false>(a, st);
+    return vec ? forward<__half, true>(a, st) : forward<__half, false>(a, st);
+}
+
+int bee_b200_norm_gate_residual_backward(int dt, const void* h, const void* x, const void* w_post, const void* gate,
+                                         const void* w_pre, const void* dx_out, const void* dy, void* dh, void* dx,
+                                         void* dw_post, void* dgate, void* dw_pre, size_t rows, size_t cols, size_t group,
+                                         float alpha, float beta, float eps, bee_b200_stream_t stream) {
+    const char* what = "norm_gate_residual_backward";
+    if (int rc = check(what, dt, rows, cols, group, gate != nullptr, alpha, beta, eps)) return rc;
+    const size_t elem = dt == DT_F32 ? 4 : 2;
+    if ((w_post && !dw_post) || (gate && !dgate) || (w_pre && !dw_pre)) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
+    cudaStream_t st = as_stream(stream);
+    if (rows == 0) {  // sums over no rows (a gate per group has no rows either)
+        cudaError_t e = cudaSuccess;
+        if (w_post) e = cudaMemsetAsync(dw_post, 0, cols * elem, st);
+        if (w_pre && e == cudaSuccess) e = cudaMemsetAsync(dw_pre, 0, cols * elem, st);
+        if (gate && group == 0 && e == cudaSuccess) e = cudaMemsetAsync(dgate, 0, cols * elem, st);
+        return e == cudaSuccess ? ok() : api_fail(e, "%s: %s", what, cudaGetErrorString(e));
+    }
+    if (!h || !x || !dh || !dx || (w_pre && !dy) || (!dx_out && !w_pre)) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
+    if (!aligned(elem, h, x, w_post, gate, w_pre, dx_out, dy, dh, dx, dw_post, dgate, dw_pre))
+        return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    NormArgs a{};
+    a.h = h; a.x = x; a.w_post = w_post; a.gate = gate; a.w_pre = w_pre;
+    a.dx_out = dx_out; a.dy = w_pre ? dy : nullptr; a.dh = dh; a.dx = dx; a.dgate = dgate;
+    a.rows = static_cast<long long>(rows);
+    a.group = static_cast<long long>(group ? group : rows);
+    a.cols = static_cast<uint32_t>(cols);
+    a.alpha = alpha; a.beta = beta; a.eps = eps;
+    const NormGrads g{w_post ? dw_post : nullptr, gate ? dgate : nullptr, w_pre ? dw_pre : nullptr};
+    const bool vec = cols * elem % 16 == 0 && aligned(16, h, x, w_post, gate, w_pre, dx_out, dy, dh, dx, gate ? dgate : nullptr);
+    if (dt == DT_F32) return vec ? backward<float, true>(a, g, st) : backward<float, false>(a, g, st);
+    if (dt == DT_BF16) return vec ? backward<__nv_bfloat16, true>(a, g, st) : backward<__nv_bfloat16, false>(a, g, st);
+    return vec ? backward<__half, true>(a, g, st) : backward<__half, false>(a, g, st);
+}
+
+}  // extern "C"

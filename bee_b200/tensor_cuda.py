@@ -176,6 +176,81 @@ def _vector(op: str, name: str, t, n: int, dtype) -> int:
     return t.data_ptr()
 
 
+def _like(op: str, name: str, t, x: torch.Tensor) -> int:
+    """Pointer of an optional contiguous tensor of x's dtype and shape."""
+    if t is None:
+        return None
+    if t.dtype != x.dtype or t.shape != x.shape or not t.is_contiguous():
+        raise BeeError(op, 1, f"{name} must be contiguous, {x.dtype}, {tuple(x.shape)}")
+    return t.data_ptr()
+
+
+def _gate(op: str, name: str, gate, rows: int, cols: int, dtype):
+    """Pointer and group of an optional gate: [cols], or [groups, cols] with groups dividing the rows."""
+    if gate is None:
+        return None, 0
+    if gate.dim() == 1:
+        return _vector(op, name, gate, cols, dtype), 0
+    if gate.dim() != 2 or gate.shape[1] != cols or gate.dtype != dtype or not gate.is_contiguous():
+        raise BeeError(op, 1, f"{name} must be contiguous, {dtype}, [cols] or [groups, cols]")
+    groups = gate.shape[0]
+    if groups == 0 and rows == 0:
+        return gate.data_ptr(), 1
+    if groups == 0 or rows % groups or rows == 0:
+        raise BeeError(op, 1, f"{rows} rows are not a multiple of {groups} gate rows")
+    return gate.data_ptr(), rows // groups
+
+
+def norm_gate_residual(h: torch.Tensor, x: torch.Tensor, x_out: torch.Tensor, y=None, *, w_post=None, gate=None,
+                       w_pre=None, alpha: float = 1.0, beta: float = 1.0, eps: float = 1e-6, stream=None, sync=False):
+    """x_out = alpha x + beta gate rmsnorm(h) w_post and y = rmsnorm(x_out) w_pre, over the last dim of [rows, cols].
+
+    w_post and w_pre [cols] and gate ([cols], or [groups, cols]: one for each rows / groups consecutive rows) are optional;
+    without w_post h is not normalised, without w_pre there is no y."""
+    op = "norm_gate_residual"
+    _current(op, h, x, x_out, y, w_post, gate, w_pre)
+    if x.dim() != 2 or not x.is_contiguous():
+        raise BeeError(op, 1, "x must be a contiguous [rows, cols] tensor")
+    rows, cols = x.shape
+    if (y is None) != (w_pre is None):
+        raise BeeError(op, 1, "y and w_pre go together")
+    gptr, group = _gate(op, "gate", gate, rows, cols, x.dtype)
+    C.call("bee_b200_norm_gate_residual", _code(x), _like(op, "h", h, x), x.data_ptr(),
+           _vector(op, "w_post", w_post, cols, x.dtype), gptr, _vector(op, "w_pre", w_pre, cols, x.dtype),
+           _like(op, "x_out", x_out, x), _like(op, "y", y, x), rows, cols, group, float(alpha), float(beta), float(eps),
+           _stream(stream))
+    _done(sync, stream)
+    return x_out
+
+
+def norm_gate_residual_backward(h: torch.Tensor, x: torch.Tensor, dx_out, dy, dh: torch.Tensor, dx: torch.Tensor, *,
+                                w_post=None, gate=None, w_pre=None, dw_post=None, dgate=None, dw_pre=None,
+                                alpha: float = 1.0, beta: float = 1.0, eps: float = 1e-6, stream=None, sync=False):
+    """Gradients dh, dx (and dw_post, dgate, dw_pre of whichever is given) from the forward's inputs and the gradients
+    dx_out (None: zero) and dy of its outputs."""
+    op = "norm_gate_residual_backward"
+    _current(op, h, x, dx_out, dy, dh, dx, w_post, gate, w_pre, dw_post, dgate, dw_pre)
+    if x.dim() != 2 or not x.is_contiguous():
+        raise BeeError(op, 1, "x must be a contiguous [rows, cols] tensor")
+    rows, cols = x.shape
+    for name, v, d in (("w_post", w_post, dw_post), ("gate", gate, dgate), ("w_pre", w_pre, dw_pre)):
+        if (v is None) != (d is None):
+            raise BeeError(op, 1, f"{name} and d{name} go together")
+    if (dy is None) != (w_pre is None):
+        raise BeeError(op, 1, "dy and w_pre go together")
+    gptr, group = _gate(op, "gate", gate, rows, cols, x.dtype)
+    if gate is not None and dgate.shape != gate.shape:
+        raise BeeError(op, 1, "dgate must have the gate's shape")
+    dgptr, _ = _gate(op, "dgate", dgate, rows, cols, x.dtype)
+    C.call("bee_b200_norm_gate_residual_backward", _code(x), _like(op, "h", h, x), x.data_ptr(),
+           _vector(op, "w_post", w_post, cols, x.dtype), gptr, _vector(op, "w_pre", w_pre, cols, x.dtype),
+           _like(op, "dx_out", dx_out, x), _like(op, "dy", dy, x), _like(op, "dh", dh, x), _like(op, "dx", dx, x),
+           _vector(op, "dw_post", dw_post, cols, x.dtype), dgptr, _vector(op, "dw_pre", dw_pre, cols, x.dtype), rows, cols,
+           group, float(alpha), float(beta), float(eps), _stream(stream))
+    _done(sync, stream)
+    return dx
+
+
 def _targets(op: str, targets, rows: int):
     if targets is None:
         return C.I64, None

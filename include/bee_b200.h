@@ -213,6 +213,36 @@ BEE_B200_API int bee_b200_softmax_rows_to(int src_dt, const void* src, int dst_d
 BEE_B200_API int bee_b200_rms_norm_rows(int dt, const void* x, const void* w, void* y, size_t rows, size_t cols,
                            float eps, bee_b200_stream_t stream);
 
+/* New: the step from one block's output to the next block's input in one pass.
+ * Over [rows, cols] h (the block's output) and x (the residual stream):
+ *   n     = h / sqrt(mean(h^2) + eps) * w_post       (n = h if w_post is NULL)
+ *   x_out = alpha * x + beta * gate * n
+ *   y     = x_out / sqrt(mean(x_out^2) + eps) * w_pre  (w_pre NULL: y is not written)
+ * w_post, w_pre: [cols].  gate: NULL (ones), [cols] for every row (group = 0), or
+ * [rows / group, cols], one for each `group` consecutive rows (e.g. a sequence).
+ * One dtype for all tensors, in {F32, BF16, F16}; math in fp32 with one rounding
+ * per output (y from the unrounded x_out); contiguous tensors, cols <= 16384
+ * (F32: 12288).  x_out may be x or h, y may be h or x (not both the same one).
+ * Fastest when cols is a whole number of 16-byte vectors and all tensors are
+ * 16-byte aligned. */
+BEE_B200_API int bee_b200_norm_gate_residual(int dt, const void* h, const void* x, const void* w_post, const void* gate,
+                                             const void* w_pre, void* x_out, void* y, size_t rows, size_t cols,
+                                             size_t group, float alpha, float beta, float eps,
+                                             bee_b200_stream_t stream);
+
+/* Its gradient: from the forward's inputs and the gradients dx_out (NULL: zero)
+ * and dy (read when w_pre is given) of its outputs, writes dh, dx [rows, cols] and,
+ * for each of w_post, gate, w_pre that is given, its gradient in its own shape
+ * (fp32 sums over the rows, rounded once).  Deterministic.  The partial sums take
+ * 16 bytes per column and CTA (at most 16 CTAs per SM) of the stream-ordered pool,
+ * returned on the stream.  dh and dx may each be any one of the inputs of their
+ * shape.  Without rows the gradients of the vectors are zeros. */
+BEE_B200_API int bee_b200_norm_gate_residual_backward(int dt, const void* h, const void* x, const void* w_post,
+                                                      const void* gate, const void* w_pre, const void* dx_out,
+                                                      const void* dy, void* dh, void* dx, void* dw_post, void* dgate,
+                                                      void* dw_pre, size_t rows, size_t cols, size_t group,
+                                                      float alpha, float beta, float eps, bee_b200_stream_t stream);
+
 /* Rotate-half RoPE on x viewed as [rows, heads, head_dim], rows = batch*seq,
  * position of row r = r % seq + pos_offset, inv_freq_i = theta^(-2i/head_dim):
  *   y[i]      = x[i] cos(p f_i) - x[i+h/2] sin(p f_i)

@@ -56,3 +56,39 @@ def logprobs_backward(dt=BF16, logits=P, ld=64, tdt=I64, targets=P, rows=4, voca
 ])
 def test_logprobs_backward_refusals(change, word):
     assert word in refused(*logprobs_backward(**change))
+
+
+def norm(dt=BF16, h=P, x=P, w_post=P, gate=P, w_pre=P, x_out=P, y=P, rows=8, cols=64, group=0, alpha=1.0, beta=1.0, eps=1e-6):
+    return ("bee_b200_norm_gate_residual", dt, h, x, w_post, gate, w_pre, x_out, y, rows, cols, group, alpha, beta, eps, None)
+
+
+def norm_backward(dt=BF16, h=P, x=P, w_post=P, gate=P, w_pre=P, dx_out=P, dy=P, dh=P, dx=P, dw_post=P, dgate=P, dw_pre=P,
+                  rows=8, cols=64, group=0, alpha=1.0, beta=1.0, eps=1e-6):
+    return ("bee_b200_norm_gate_residual_backward", dt, h, x, w_post, gate, w_pre, dx_out, dy, dh, dx, dw_post, dgate,
+            dw_pre, rows, cols, group, alpha, beta, eps, None)
+
+
+@pytest.mark.parametrize("call", [norm, norm_backward])
+@pytest.mark.parametrize("change,word", [
+    ({"dt": I32}, "dtype"), ({"h": None}, "null"), ({"x": None}, "null"), ({"cols": 0}, "columns"), ({"cols": 16385}, "columns"),
+    ({"dt": F32, "cols": 12289}, "columns"), ({"group": 3}, "group"), ({"eps": -1.0}, "eps"), ({"eps": math.nan}, "eps"),
+    ({"eps": math.inf}, "eps"), ({"alpha": math.nan}, "alpha"), ({"beta": math.inf}, "alpha"), ({"x": P + 1}, "aligned"),
+    ({"gate": P + 1}, "aligned"),
+])
+def test_norm_refusals(call, change, word):
+    assert word in refused(*call(**change))
+
+
+def test_norm_forward_refusals():
+    assert "null" in refused(*norm(x_out=None))
+    assert "null" in refused(*norm(y=None))
+    accepted(*norm(rows=0, h=None, x=None, x_out=None, y=None))
+
+
+@pytest.mark.parametrize("missing", ["dh", "dx", "dy", "dw_post", "dgate", "dw_pre"])
+def test_norm_backward_refusals(missing):
+    assert "null" in refused(*norm_backward(**{missing: None}))
+
+
+def test_norm_backward_needs_a_gradient():
+    assert "null" in refused(*norm_backward(w_pre=None, dw_pre=None, dy=None, dx_out=None))
