@@ -74,6 +74,9 @@ SIGNATURES = {
     "bee_b200_bmm": [_i, _i, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _i, _f, _vp],
     "bee_b200_bmm_strided": [_i, _i, _vp, _c.c_int64, _c.c_int64, _vp, _c.c_int64, _c.c_int64, _vp, _c.c_int64,
                              _c.c_int64, _sz, _sz, _sz, _sz, _i, _f, _vp],
+    "bee_b200_gated_linear": [_i, _i, _vp, _sz, _vp, _vp, _sz, _i, _vp, _vp, _vp, _sz, _sz, _sz, _vp],
+    "bee_b200_gated_linear_backward": [_i, _i, _vp, _sz, _vp, _vp, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz,
+                                       _sz, _vp],
     "bee_b200_attention": [_i, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _f, _vp],
     "bee_b200_transpose_2d": [_i, _vp, _vp, _sz, _sz, _vp],
     "bee_b200_strided_copy": [_i, _vp, _i, _c.POINTER(_c.c_int64), _c.POINTER(_c.c_int64), _vp, _vp],

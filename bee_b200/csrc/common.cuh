@@ -121,6 +121,8 @@ cudaError_t pool_malloc(void** ptr, size_t bytes, cudaStream_t st);
 int attention_status_take(int* code);
 // Reads and clears the status word of the cross-GPU reduce (a peer that never arrived).
 int allranks_status_take(int* code);
+// Reads and clears the status word of the gated linear kernels.
+int gated_linear_status_take(int* code);
 
 inline cudaStream_t as_stream(bee_b200_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 

@@ -282,11 +282,17 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t lbo_byt
 // Instruction descriptor for kind::f16 with fp32 D and 16-bit A/B (both bf16
 // or both f16 — one MMA never mixes them):
 //   bits 4-5 D format (1 = f32), 7-9 A format and 10-12 B format (0 = f16,
-//   1 = bf16), bit 15 A major (0 = K), bit 16 B major (1 = MN), bits 17-22
+//   1 = bf16), bit 15 A major (0 = K, 1 = MN), bit 16 B major (1 = MN), bits 17-22
 //   N >> 3, bits 24-28 M >> 4.
 __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t m, uint32_t n, bool b_mn_major, bool f16_inputs) {
     return (1u << 4) | ((f16_inputs ? 0u : 1u) << 7) | ((f16_inputs ? 0u : 1u) << 10) |
            ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// The same with A stored MN-major too (bit 15).
+__host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t m, uint32_t n, bool a_mn_major, bool b_mn_major,
+                                                     bool f16_inputs) {
+    return idesc_f16_f32(m, n, b_mn_major, f16_inputs) | ((a_mn_major ? 1u : 0u) << 15);
 }
 
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(uint32_t m, uint32_t n, bool b_mn_major) {

@@ -311,3 +311,77 @@ def token_logprobs_backward(logits: torch.Tensor, targets, row_max: torch.Tensor
            _vector(op, "dentropy", dentropy, rows, f32), dlogits.data_ptr(), ldd, _stream(stream))
     _done(sync, stream)
     return dlogits
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def _act(op: str, act: str) -> int:
+    try:
+        return ACTIVATIONS[act]
+    except KeyError:
+        raise BeeError(op, 1, f"act must be one of {', '.join(ACTIVATIONS)}") from None
+
+
+def _pair(op: str, names: str, a: torch.Tensor, b: torch.Tensor, shape, dtype) -> int:
+    """Common row stride of two matrices of one shape."""
+    ld = _rows(op, names, a)
+    if _rows(op, names, b) != ld or a.shape != shape or b.shape != shape or a.dtype != dtype or b.dtype != dtype:
+        raise BeeError(op, 1, f"{names} must both be {dtype}, {tuple(shape)}, with the same row stride")
+    return ld
+
+
+def _matrix(op: str, name: str, t, m: int, n: int, dtype) -> int:
+    """Pointer of an optional contiguous [m, n] matrix."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != (m, n) or not t.is_contiguous():
+        raise BeeError(op, 1, f"{name} must be contiguous, {dtype}, ({m}, {n})")
+    return t.data_ptr()
+
+
+def gated_linear(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, out: torch.Tensor, *, act: str = "silu",
+                 trans: bool = False, g=None, u=None, stream=None, sync=False):
+    """out = act(x @ wg) * (x @ wu): x [M, D], out [M, F]; wg and wu [D, F], or [F, D] with trans.
+
+    x and the weights may have strided rows.  act is "silu", "gelu" or "gelu_tanh".  g and u [M, F], when given, receive
+    the two products for the backward."""
+    op = "gated_linear"
+    _current(op, x, wg, wu, out, g, u)
+    ldx = _rows(op, "x", x)
+    m, d = x.shape
+    f = out.shape[-1]
+    ldw = _pair(op, "wg and wu", wg, wu, (f, d) if trans else (d, f), x.dtype)
+    if (g is None) != (u is None):
+        raise BeeError(op, 1, "g and u go together")
+    C.call("bee_b200_gated_linear", _code(x), _act(op, act), x.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw, int(trans),
+           _matrix(op, "out", out, m, f, x.dtype), _matrix(op, "g", g, m, f, x.dtype), _matrix(op, "u", u, m, f, x.dtype), m, d,
+           f, _stream(stream))
+    _done(sync, stream)
+    return out
+
+
+def gated_linear_backward(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, g: torch.Tensor, u: torch.Tensor,
+                          dout: torch.Tensor, dx=None, dwg=None, dwu=None, *, act: str = "silu", trans: bool = False,
+                          stream=None, sync=False):
+    """Gradients dx [M, D] and dwg, dwu (in the weights' layout; rows may be strided) from the forward's inputs, its g and
+    u, and dout [M, F].  dx, or dwg and dwu, may be None."""
+    op = "gated_linear_backward"
+    _current(op, x, wg, wu, g, u, dout, dx, dwg, dwu)
+    ldx = _rows(op, "x", x)
+    m, d = x.shape
+    f = g.shape[-1]
+    shape = (f, d) if trans else (d, f)
+    ldw = _pair(op, "wg and wu", wg, wu, shape, x.dtype)
+    if (dwg is None) != (dwu is None):
+        raise BeeError(op, 1, "dwg and dwu go together")
+    if dx is None and dwg is None:
+        raise BeeError(op, 1, "no gradient is asked for")
+    lddw = _pair(op, "dwg and dwu", dwg, dwu, shape, x.dtype) if dwg is not None else 0
+    C.call("bee_b200_gated_linear_backward", _code(x), _act(op, act), x.data_ptr(), ldx, wg.data_ptr(), wu.data_ptr(), ldw,
+           int(trans), _matrix(op, "g", g, m, f, x.dtype), _matrix(op, "u", u, m, f, x.dtype),
+           _matrix(op, "dout", dout, m, f, x.dtype), _matrix(op, "dx", dx, m, d, x.dtype),
+           dwg.data_ptr() if dwg is not None else None, dwu.data_ptr() if dwu is not None else None, lddw, m, d, f,
+           _stream(stream))
+    _done(sync, stream)
+    return dx

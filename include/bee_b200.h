@@ -340,6 +340,34 @@ BEE_B200_API int bee_b200_bmm_strided(int dt_in, int dt_out, const void* A, int6
                                       size_t batch, size_t M, size_t K, size_t N, int b_trans, float alpha,
                                       bee_b200_stream_t stream);
 
+/* New: the first half of a gated feed-forward block,
+ *   out = act(x Wg) * (x Wu),
+ * both products, the activation and the elementwise product in one kernel.
+ * x [M, D] (row stride ldx), out [M, F] contiguous; Wg and Wu [D, F], or [F, D]
+ * when trans != 0 (as a Linear layer keeps them), both with row stride ldw, so
+ * they may be two slices of one fused matrix.  g and u (both or neither, [M, F]
+ * contiguous): x Wg and x Wu, kept for the backward.  act: 0 silu, 1 gelu (erf),
+ * 2 gelu (tanh).  dt in {BF16, F16}; fp32 accumulation on the tensor cores, one
+ * rounding per output (out from the unrounded products).  Up to 128 rows run a
+ * kernel that is bound by reading the weights once.  Operands whose rows are not 16-byte
+ * aligned are copied to padded scratch first (2 bytes an element of them, from
+ * the stream-ordered pool). */
+BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ldx, const void* wg, const void* wu,
+                                       size_t ldw, int trans, void* out, void* g, void* u, size_t M, size_t D,
+                                       size_t F, bee_b200_stream_t stream);
+
+/* Its gradient, from x, the weights, the forward's g and u and dout (g, u, dout
+ * [M, F] contiguous):  dg = dout u act'(g) and du = dout act(g), rounded to dt;
+ * dx = dg Wg^T + du Wu^T [M, D] contiguous; dwg = x^T dg and dwu = x^T du in the
+ * weights' layout with row stride lddw.  dx may be NULL (then the weights are
+ * not read), or dwg and dwu (then x is not).  Deterministic.  Takes 4*M*F bytes of
+ * pool scratch (F rounded up to 8), plus the copies of unaligned operands as above.  Without rows
+ * dwg and dwu are zeros. */
+BEE_B200_API int bee_b200_gated_linear_backward(int dt, int act, const void* x, size_t ldx, const void* wg,
+                                                const void* wu, size_t ldw, int trans, const void* g, const void* u,
+                                                const void* dout, void* dx, void* dwg, void* dwu, size_t lddw,
+                                                size_t M, size_t D, size_t F, bee_b200_stream_t stream);
+
 /* Fused attention forward, per head: O = softmax(Q.K^T * scale) . V with
  * fp32 scores, softmax and accumulation; Q, K, V, O are [heads, seq, head_dim]
  * bf16, contiguous, 16-byte aligned.  One pass: scores and probabilities stay

@@ -92,3 +92,40 @@ def test_norm_backward_refusals(missing):
 
 def test_norm_backward_needs_a_gradient():
     assert "null" in refused(*norm_backward(w_pre=None, dw_pre=None, dy=None, dx_out=None))
+
+
+def gated(dt=BF16, act=0, x=P, ldx=64, wg=P, wu=P, ldw=96, trans=0, out=P, g=None, u=None, M=8, D=64, F=96):
+    return ("bee_b200_gated_linear", dt, act, x, ldx, wg, wu, ldw, trans, out, g, u, M, D, F, None)
+
+
+def gated_backward(dt=BF16, act=0, x=P, ldx=64, wg=P, wu=P, ldw=96, trans=0, g=P, u=P, dout=P, dx=P, dwg=P, dwu=P, lddw=96,
+                   M=8, D=64, F=96):
+    return ("bee_b200_gated_linear_backward", dt, act, x, ldx, wg, wu, ldw, trans, g, u, dout, dx, dwg, dwu, lddw, M, D, F, None)
+
+
+@pytest.mark.parametrize("call", [gated, gated_backward])
+@pytest.mark.parametrize("change,word", [
+    ({"dt": F32}, "dtype"), ({"act": 3}, "activation"), ({"act": -1}, "activation"), ({"D": 0}, "extents"), ({"F": 0}, "extents"),
+    ({"M": 2 ** 31}, "extents"), ({"F": 2 ** 31, "ldw": 2 ** 31}, "extents"), ({"ldx": 63}, "stride"), ({"ldw": 95}, "stride"),
+    ({"ldw": 63, "trans": 1}, "stride"), ({"x": None}, "null"), ({"wg": None}, "null"), ({"wu": None}, "null"), ({"x": P + 1}, "aligned"),
+    ({"wu": P + 1}, "aligned"),
+])
+def test_gated_refusals(call, change, word):
+    assert word in refused(*call(**change))
+
+
+def test_gated_forward_refusals():
+    assert "null" in refused(*gated(out=None))
+    assert "null" in refused(*gated(g=P))
+    accepted(*gated(M=0, x=None, wg=None, wu=None, out=None))
+
+
+@pytest.mark.parametrize("change", [{"g": None}, {"u": None}, {"dout": None}, {"dwg": None}, {"dwu": None},
+                                    {"dx": None, "dwg": None, "dwu": None}])
+def test_gated_backward_refusals(change):
+    assert "null" in refused(*gated_backward(**change))
+
+
+def test_gated_backward_stride():
+    assert "stride" in refused(*gated_backward(lddw=95))
+    accepted(*gated_backward(M=0, dwg=None, dwu=None, x=None, wg=None, wu=None, g=None, u=None, dout=None))
