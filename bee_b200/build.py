@@ -37,6 +37,8 @@ CUDA_INC = str(Path(NVCC).resolve().parent.parent / "include")
 HOST_FLAGS = ["-O2", "-std=c++23", "-fPIC", "-I", str(ROOT / "include"), "-I", str(HOST), "-I", CUDA_INC]
 HOST_TEST_SRC = ROOT / "tests" / "cpp" / "test_host_bridge.cpp"
 HOST_TEST_BIN = LIB_DIR / "test_host_bridge"
+BLOCK_TEST_SRC = HOST_TEST_SRC.with_name("test_host_bridge_block.cpp")
+BLOCK_TEST_BIN = LIB_DIR / "test_host_bridge_block"
 BRIDGE_BENCH_SRC = HOST / "bridge_bench.cpp"
 BRIDGE_BENCH_BIN = LIB_DIR / "bridge_bench"
 
@@ -83,10 +85,11 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         objs.append(obj)
     if force or _stale(LIB, objs):
         _run([NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objs), "-lrt", "-ldl", "-lpthread"])
-    # C++ program exercising the host bridge (run by tests/test_gpu_host_bridge.py)
-    if HOST_TEST_SRC.exists() and (force or _stale(HOST_TEST_BIN, [HOST_TEST_SRC, LIB] + headers)):
-        _run(["g++", *HOST_FLAGS, str(HOST_TEST_SRC), "-o", str(HOST_TEST_BIN), "-L", str(LIB_DIR), "-lbee_b200",
-              "-Wl,-rpath,$ORIGIN"])
+    # C++ programs exercising the host bridge (run by tests/test_gpu_host_bridge.py and tests/test_gpu_block.py)
+    for test_src, test_bin in ((HOST_TEST_SRC, HOST_TEST_BIN), (BLOCK_TEST_SRC, BLOCK_TEST_BIN)):
+        if test_src.exists() and (force or _stale(test_bin, [test_src, LIB] + headers)):
+            _run(["g++", *HOST_FLAGS, str(test_src), "-o", str(test_bin), "-L", str(LIB_DIR), "-lbee_b200",
+                  "-Wl,-rpath,$ORIGIN"])
     # measurement program for the bridge's plumbing cost (run by bench.py)
     if BRIDGE_BENCH_SRC.exists() and (force or _stale(BRIDGE_BENCH_BIN, [BRIDGE_BENCH_SRC, LIB] + headers)):
         _run(["g++", *HOST_FLAGS, str(BRIDGE_BENCH_SRC), "-o", str(BRIDGE_BENCH_BIN), "-L", str(LIB_DIR),

@@ -198,4 +198,54 @@ auto attention(int dt, const void* q, const void* k, const void* v, void* o, std
                   "cuda::ops::attention");
 }
 
+auto norm_gate_residual(int dt, const void* h, const void* x, const void* w_post, const void* gate, const void* w_pre,
+                        void* x_out, void* y, std::size_t rows, std::size_t cols, std::size_t group, float alpha, float beta,
+                        float eps) -> Result<void> {
+    return finish(bee_b200_norm_gate_residual(dt, h, x, w_post, gate, w_pre, x_out, y, rows, cols, group, alpha, beta, eps,
+                                              per_thread_stream()),
+                  "cuda::ops::norm_gate_residual");
+}
+
+auto norm_gate_residual_backward(int dt, const void* h, const void* x, const void* w_post, const void* gate,
+                                 const void* w_pre, const void* dx_out, const void* dy, void* dh, void* dx, void* dw_post,
+                                 void* dgate, void* dw_pre, std::size_t rows, std::size_t cols, std::size_t group,
+                                 float alpha, float beta, float eps) -> Result<void> {
+    return finish(bee_b200_norm_gate_residual_backward(dt, h, x, w_post, gate, w_pre, dx_out, dy, dh, dx, dw_post, dgate,
+                                                       dw_pre, rows, cols, group, alpha, beta, eps, per_thread_stream()),
+                  "cuda::ops::norm_gate_residual_backward");
+}
+
+auto gated_linear(int dt, int act, const void* x, std::size_t ldx, const void* wg, const void* wu, std::size_t ldw,
+                  bool w_transposed, void* out, void* g, void* u, std::size_t M, std::size_t D, std::size_t F)
+    -> Result<void> {
+    return finish(bee_b200_gated_linear(dt, act, x, ldx, wg, wu, ldw, w_transposed ? 1 : 0, out, g, u, M, D, F,
+                                        per_thread_stream()),
+                  "cuda::ops::gated_linear");
+}
+
+auto gated_linear_backward(int dt, int act, const void* x, std::size_t ldx, const void* wg, const void* wu, std::size_t ldw,
+                           bool w_transposed, const void* g, const void* u, const void* dout, void* dx, void* dwg,
+                           void* dwu, std::size_t lddw, std::size_t M, std::size_t D, std::size_t F) -> Result<void> {
+    return finish(bee_b200_gated_linear_backward(dt, act, x, ldx, wg, wu, ldw, w_transposed ? 1 : 0, g, u, dout, dx, dwg,
+                                                 dwu, lddw, M, D, F, per_thread_stream()),
+                  "cuda::ops::gated_linear_backward");
+}
+
+auto token_logprobs(int dt, const void* logits, std::size_t ld, int targets_dt, const void* targets, std::size_t rows,
+                    std::size_t vocab, float temperature, float* logprob, float* entropy, float* row_max, float* log_sum,
+                    std::size_t top, std::int32_t* top_ids, float* top_logprobs) -> Result<void> {
+    return finish(bee_b200_token_logprobs(dt, logits, ld, targets_dt, targets, rows, vocab, temperature, logprob, entropy,
+                                          row_max, log_sum, top, top_ids, top_logprobs, per_thread_stream()),
+                  "cuda::ops::token_logprobs");
+}
+
+auto token_logprobs_backward(int dt, const void* logits, std::size_t ld, int targets_dt, const void* targets,
+                             std::size_t rows, std::size_t vocab, float temperature, const float* row_max,
+                             const float* log_sum, const float* entropy, const float* dlogprob, const float* dentropy,
+                             void* dlogits, std::size_t ldd) -> Result<void> {
+    return finish(bee_b200_token_logprobs_backward(dt, logits, ld, targets_dt, targets, rows, vocab, temperature, row_max,
+                                                   log_sum, entropy, dlogprob, dentropy, dlogits, ldd, per_thread_stream()),
+                  "cuda::ops::token_logprobs_backward");
+}
+
 }  // namespace bee_b200::tensor_cuda

@@ -95,6 +95,35 @@ auto deallocate(void* p, std::size_t nbytes, std::size_t alignment) -> void;
                                  std::size_t heads, std::size_t head_dim, float eps, double theta,
                                  std::size_t pos_offset) -> Result<void>;
 
+// x_out = alpha x + beta gate rmsnorm(h) w_post and y = rmsnorm(x_out) w_pre over [rows, cols], and its gradient
+// (bee_b200.h; w_post, gate, w_pre and their gradients null when absent, group 0 for one gate row)
+[[nodiscard]] auto norm_gate_residual(int dt, const void* h, const void* x, const void* w_post, const void* gate,
+                                      const void* w_pre, void* x_out, void* y, std::size_t rows, std::size_t cols,
+                                      std::size_t group, float alpha, float beta, float eps) -> Result<void>;
+[[nodiscard]] auto norm_gate_residual_backward(int dt, const void* h, const void* x, const void* w_post, const void* gate,
+                                               const void* w_pre, const void* dx_out, const void* dy, void* dh, void* dx,
+                                               void* dw_post, void* dgate, void* dw_pre, std::size_t rows,
+                                               std::size_t cols, std::size_t group, float alpha, float beta, float eps)
+    -> Result<void>;
+// out = act(x Wg) * (x Wu), x [M, D], weights [D, F] ([F, D] when transposed), and its gradient
+[[nodiscard]] auto gated_linear(int dt, int act, const void* x, std::size_t ldx, const void* wg, const void* wu,
+                                std::size_t ldw, bool w_transposed, void* out, void* g, void* u, std::size_t M,
+                                std::size_t D, std::size_t F) -> Result<void>;
+[[nodiscard]] auto gated_linear_backward(int dt, int act, const void* x, std::size_t ldx, const void* wg, const void* wu,
+                                         std::size_t ldw, bool w_transposed, const void* g, const void* u,
+                                         const void* dout, void* dx, void* dwg, void* dwu, std::size_t lddw,
+                                         std::size_t M, std::size_t D, std::size_t F) -> Result<void>;
+// log probabilities of targets under softmax(logits / temperature), entropy and top alternatives, and the gradient
+[[nodiscard]] auto token_logprobs(int dt, const void* logits, std::size_t ld, int targets_dt, const void* targets,
+                                  std::size_t rows, std::size_t vocab, float temperature, float* logprob, float* entropy,
+                                  float* row_max, float* log_sum, std::size_t top, std::int32_t* top_ids,
+                                  float* top_logprobs) -> Result<void>;
+[[nodiscard]] auto token_logprobs_backward(int dt, const void* logits, std::size_t ld, int targets_dt,
+                                           const void* targets, std::size_t rows, std::size_t vocab, float temperature,
+                                           const float* row_max, const float* log_sum, const float* entropy,
+                                           const float* dlogprob, const float* dentropy, void* dlogits, std::size_t ldd)
+    -> Result<void>;
+
 // fused O = softmax(scale * Q K^T) V per head: q, k, v, o [heads, seq, head_dim] bf16
 [[nodiscard]] auto attention(int dt, const void* q, const void* k, const void* v, void* o, std::size_t heads,
                              std::size_t seq, std::size_t head_dim, float scale) -> Result<void>;
