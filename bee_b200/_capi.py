@@ -116,7 +116,7 @@ def lib() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls a status-returning entry point and raises BeeError on failure."""
-    h = lib()
+    h = _lib or lib()
     rc = getattr(h, name)(*args)
     if rc != 0:
         msg = h.bee_b200_last_error().decode(errors="replace")

@@ -150,7 +150,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0
 
 // Moves the sums from maximum st.m to maximum m (>= st.m).
 __device__ __forceinline__ void rebase(Stat& st, float m, float c) {
-    if (st.s != 0.f) {  // s is 0 only while the maximum is -inf; a NaN stays
+    if (st.s != 0.f && st.m != m) {  // s is 0 only while the maximum is -inf; a NaN stays
         const float d = fmaxf((st.m - m) * c, kZFloor);
         const float r = ex2(d);
         st.z = r * fmaf(d, st.s, st.z);
@@ -159,11 +159,12 @@ __device__ __forceinline__ void rebase(Stat& st, float m, float c) {
     st.m = m;
 }
 
-__device__ __forceinline__ Stat join(Stat a, Stat b, float c) {
-    const float m = fmaxf(a.m, b.m);
-    if (a.m != m) rebase(a, m, c);
-    if (b.m != m) rebase(b, m, c);
-    return Stat{m, a.s + b.s, a.z + b.z};
+// The warp's statistics, in every lane: one maximum, then each lane's sums moved to it and added.
+__device__ __forceinline__ Stat warp_join(Stat st, float c) {
+    rebase(st, warp_max(st.m), c);
+    st.s = warp_sum(st.s);
+    st.z = warp_sum(st.z);
+    return st;
 }
 
 // ---------------------------------------------------------------- keys
@@ -233,38 +234,103 @@ __device__ __forceinline__ long long target_of(const void* t, int is64, long lon
     return is64 ? static_cast<const long long*>(t)[r] : static_cast<const int*>(t)[r];
 }
 
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 4;  // chunks of a thread per batch
+constexpr int kMaxCluster = 8;
+constexpr int kStages = 3;  // batches in its part of the shared-memory ring
 
-// Rows in grid-stride order (cluster == 1), or one row per cluster of `cluster`
-// CTAs, each taking a contiguous range of the row's chunks.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
+}
+
+// One CTA's part of a row: the whole chunks [lo, hi) and perhaps the partial
+// first or last chunk of the row.
+template <typename T> struct Part {
+    RowChunks<T> row;
+    int lo, hi, edge_lo, edge_hi;  // edge_lo, edge_hi: index of the partial chunk, or -1
+    __device__ __forceinline__ Part(const LogprobArgs& a, long long r, int rank, int cluster)
+        : row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab) {
+        const int whole = max(row.full_hi - row.full_lo, 0), per = (whole + cluster - 1) / cluster;
+        lo = row.full_lo + min(whole, rank * per);
+        hi = row.full_lo + min(whole, (rank + 1) * per);
+        edge_lo = rank == 0 && row.full_lo > 0 ? 0 : -1;
+        edge_hi = rank == cluster - 1 && row.full_hi < row.chunks && row.full_hi >= row.full_lo ? row.full_hi : -1;
+    }
+    // the thread that reads chunk c
+    template <int THREADS> __device__ __forceinline__ int owner(int c) const {
+        return c == edge_lo ? 0 : c == edge_hi ? 1 : (c - lo) % THREADS;
+    }
+};
+
+// Clusters of `cluster` CTAs (1: single CTAs) take rows in grid-stride order.
+// Every thread streams its own chunks of the coming batches, across rows, into
+// its own slots of a ring with cp.async, so that loads stay in flight while a row
+// is joined and its alternatives are sought; no barrier is needed for the ring.
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobArgs a, int cluster) {
     constexpr int WARPS = THREADS / 32;
+    static_assert(2 * WARPS >= kMaxCluster, "a warp of rank 0 joins at most two of the cluster's lists");
     constexpr int E = Elems<T>::E;
+    extern __shared__ __align__(16) uint4 ring[];  // [kStages][kUnroll][THREADS]
     __shared__ Stat warp_stat[WARPS];
-    __shared__ Stat cta_stat[8];                 // rank 0's copy is filled by the whole cluster
+    __shared__ Stat cta_stat[2][kMaxCluster];                // rank 0's copy is filled by the whole cluster, alternating by row
     __shared__ uint64_t lists[WARPS][32];
-    __shared__ uint64_t cta_list[TOP ? 8 : 1][32];
+    __shared__ uint64_t cta_list[2][TOP ? kMaxCluster : 1][32];
     __shared__ uint64_t owners[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = cluster > 1 ? static_cast<int>(sm100::cluster_ctarank()) : 0;
     const float c = a.inv_t * kLog2e;
     if (cluster > 1) sm100::cluster_sync();  // every CTA of the cluster runs before its shared memory is written
     pdl_wait();
-    const long long step = gridDim.x / cluster;
-    for (long long r = blockIdx.x / cluster; r < a.rows; r += step) {
-        if (r + step >= a.rows) pdl_trigger();  // this CTA's last row
-        const RowChunks<T> row(static_cast<const T*>(a.logits) + r * a.ld, a.vocab);
-        const int per = (row.chunks + cluster - 1) / cluster;
-        const int c_begin = min(row.chunks, rank * per), c_end = min(row.chunks, c_begin + per);
+    const long long step = gridDim.x / cluster, r0 = blockIdx.x / cluster;
 
-        // the target's logit: one early load by the thread that writes the row's results
+    // the batch to copy next: the issue_at-th chunk of issue_row's part onwards
+    long long issue_row = r0;
+    int issue_at = tid, issue_hi = 0, issue_slot = 0;
+    const uint4* issue_base = nullptr;
+    int issue_end = 0;  // uniform: batches left in the row
+    auto open_row = [&] {
+        if (issue_row >= a.rows) return;
+        const Part<T> p(a, issue_row, rank, cluster);
+        issue_base = p.row.base;
+        issue_at = p.lo + tid;
+        issue_hi = p.hi;
+        issue_end = (p.hi - p.lo + kUnroll * THREADS - 1) / (kUnroll * THREADS);
+    };
+    auto issue = [&] {
+        while (issue_row < a.rows && issue_end == 0) {  // rows without whole chunks have no batches
+            issue_row += step;
+            open_row();
+        }
+        if (issue_row < a.rows) {
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j)
+                if (issue_at + j * THREADS < issue_hi)
+                    cp_async16(ring + (issue_slot * kUnroll + j) * THREADS + tid, issue_base + issue_at + j * THREADS);
+            issue_at += kUnroll * THREADS;
+            --issue_end;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");  // empty past the end: the wait counts stay uniform
+        issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
+    };
+    open_row();
+    for (int j = 1; j < kStages; ++j) issue();
+
+    int slot = 0, turn = 0;
+    for (long long r = r0; r < a.rows; r += step, turn ^= 1) {
+        if (r + step >= a.rows) pdl_trigger();  // this CTA's last row
+        const Part<T> part(a, r, rank, cluster);
+        const RowChunks<T>& row = part.row;
+
+        // early loads: the target's logit (by the thread that writes the row's results) and the partial chunks
         long long target = -1;
         float xt = -INFINITY;
         if (tid == 0 && rank == 0 && a.logprob) {
             target = target_of(a.targets, a.targets_i64, r);
             xt = target < 0 ? 0.f : target < a.vocab ? Elems<T>::get(row.row + target) : NAN;
         }
+        const int edge = tid == 0 ? part.edge_lo : tid == 1 ? part.edge_hi : -1;
+        uint4 edge_chunk = Elems<T>::fill();
+        if (edge >= 0) edge_chunk = row.partial(edge);
 
         Stat st{-INFINITY, 0.f, 0.f};
         int at = -1;  // the chunk that holds this thread's maximum
@@ -275,15 +341,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 cm[j] = Elems<T>::max(q[j]);
                 bm = fmaxf(bm, cm[j]);
             }
-            if (bm > st.m || at < 0) {
+            // the partial first chunk comes last but holds the lowest indices: it wins a tie
+            if (bm > st.m || at < 0 || (TOP && c0 == part.edge_lo && bm == st.m)) {
                 rebase(st, bm, c);
+                at = c0;
                 if (TOP) {
-                    at = c0;
 #pragma unroll
                     for (int j = kUnroll - 1; j >= 0; --j)
                         if (j < count && cm[j] == bm) at = c0 + j * THREADS;
-                } else {
-                    at = 0;
                 }
             }
             const float m = finite_max(st.m);
@@ -310,31 +375,34 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             unpack_f32x2(z2, lo, hi);
             st.z += lo + hi;
         };
-        int ch = c_begin + tid;
-        for (; ch + (kUnroll - 1) * THREADS < c_end; ch += kUnroll * THREADS) {
+        for (int c0 = part.lo; c0 < part.hi; c0 += kUnroll * THREADS) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            issue();
+            const uint4* mine = ring + slot * kUnroll * THREADS + tid;
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            const int left = part.hi - c0 - tid;  // this thread's chunks are those at 0, THREADS, ... below `left`
+            if (left <= 0) continue;
             uint4 q[kUnroll];
-            if (row.whole(ch) && row.whole(ch + (kUnroll - 1) * THREADS)) {
+            if (left > (kUnroll - 1) * THREADS) {
 #pragma unroll
-                for (int j = 0; j < kUnroll; ++j) q[j] = TOP ? __ldg(row.base + ch + j * THREADS) : __ldcs(row.base + ch + j * THREADS);
+                for (int j = 0; j < kUnroll; ++j) q[j] = mine[j * THREADS];
+                consume(q, c0 + tid, kUnroll);
             } else {
 #pragma unroll
-                for (int j = 0; j < kUnroll; ++j) q[j] = row.load(ch + j * THREADS);
+                for (int j = 0; j < kUnroll; ++j) q[j] = j * THREADS < left ? mine[j * THREADS] : Elems<T>::fill();
+                consume(q, c0 + tid, (left + THREADS - 1) / THREADS);
             }
-            consume(q, ch, kUnroll);
         }
-        if (ch < c_end) {  // fewer than kUnroll chunks are left to this thread
+        if (edge >= 0) {
             uint4 q[kUnroll];
-            int count = 0;
+            q[0] = edge_chunk;
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                const bool in = ch + j * THREADS < c_end;
-                q[j] = in ? row.load(ch + j * THREADS) : Elems<T>::fill();
-                count += in;
-            }
-            consume(q, ch, count);
+            for (int j = 1; j < kUnroll; ++j) q[j] = Elems<T>::fill();
+            consume(q, edge, 1);
         }
+        __syncwarp();
 
-        uint64_t mine = 0;
+        uint64_t best = 0;
         if constexpr (TOP) {
             // owners of the k largest thread maxima
             uint64_t key = at >= 0 ? make_key(st.m, static_cast<uint32_t>(at)) : 0;
@@ -342,67 +410,66 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             if (warp == 0) owners[lane] = key;
             __syncthreads();
             const uint32_t bound = static_cast<uint32_t>(owners[a.top - 1] >> 32);  // 0 if fewer threads hold anything
+            // inserts the elements of each lane's chunk (index cc; none where !in) into the warp's sorted list
+            auto insert = [&](uint4 chunk, int cc, bool in) {
+                float v[E];
+                Elems<T>::unpack(chunk, v);
+                const long long i0 = row.first(cc);
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const bool real = in && i0 + e >= 0 && i0 + e < row.n && v[e] == v[e] && ordered(v[e]) >= bound;
+                    if (!__any_sync(0xffffffffu, real)) continue;
+                    const uint64_t ck = real ? make_key(v[e], static_cast<uint32_t>(i0 + e)) : 0;
+                    uint32_t todo = __ballot_sync(0xffffffffu, ck > __shfl_sync(0xffffffffu, best, 31));
+                    while (todo) {
+                        const int src = __ffs(todo) - 1;
+                        todo &= todo - 1;
+                        const uint64_t nk = __shfl_sync(0xffffffffu, ck, src);
+                        const int pos = __popc(__ballot_sync(0xffffffffu, best > nk));
+                        const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
+                        best = lane < pos ? best : lane == pos ? nk : up;
+                    }
+                }
+            };
             for (int j = warp; j < a.top; j += WARPS) {
                 const uint64_t o = owners[j];
                 if (o == 0) break;  // the list is sorted: no more owners
-                const int owner = static_cast<int>((~static_cast<uint32_t>(o)) - static_cast<uint32_t>(c_begin)) % THREADS;
-                for (int cb = c_begin + owner; cb < c_end; cb += 32 * THREADS) {
+                const int owner = part.template owner<THREADS>(static_cast<int>(~static_cast<uint32_t>(o)));
+                for (int cb = part.lo + owner; cb < part.hi; cb += 32 * THREADS) {
                     const int cc = cb + lane * THREADS;
-                    float v[E];
-                    Elems<T>::unpack(cc < c_end ? row.load(cc) : Elems<T>::fill(), v);
-                    const long long i0 = row.first(cc);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const bool real = cc < c_end && i0 + e >= 0 && i0 + e < row.n && v[e] == v[e];
-                        const uint64_t ck = real && ordered(v[e]) >= bound ? make_key(v[e], static_cast<uint32_t>(i0 + e)) : 0;
-                        uint32_t todo = __ballot_sync(0xffffffffu, ck > __shfl_sync(0xffffffffu, mine, 31));
-                        while (todo) {
-                            const int src = __ffs(todo) - 1;
-                            todo &= todo - 1;
-                            const uint64_t nk = __shfl_sync(0xffffffffu, ck, src);
-                            const int pos = __popc(__ballot_sync(0xffffffffu, mine > nk));
-                            const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
-                            mine = lane < pos ? mine : lane == pos ? nk : up;
-                        }
-                    }
+                    insert(cc < part.hi ? __ldg(row.base + cc) : Elems<T>::fill(), cc, cc < part.hi);
                 }
+                const int partial = owner == 0 ? part.edge_lo : owner == 1 ? part.edge_hi : -1;
+                if (partial >= 0) insert(lane == 0 ? row.partial(partial) : Elems<T>::fill(), partial, lane == 0);
             }
         }
 
-        // join the block's statistics in a fixed order
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Stat other{__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
-                             __shfl_xor_sync(0xffffffffu, st.z, o)};
-            st = (lane & o) ? join(other, st, c) : join(st, other, c);
-        }
+        // join the block's statistics, then the cluster's, each in a fixed order
+        st = warp_join(st, c);
         if (lane == 0) warp_stat[warp] = st;
-        if constexpr (TOP) mine = merge_block<WARPS>(mine, lists, warp, lane);
+        if constexpr (TOP) best = merge_block<WARPS>(best, lists, warp, lane);
         __syncthreads();
-        if (warp == 0) {
-            st = warp_stat[0];
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) st = join(st, warp_stat[w], c);
-        }
+        if (warp == 0) st = warp_join(lane < WARPS ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f}, c);
         if (cluster > 1) {
             if (warp == 0) {
-                const uint32_t dst = sm100::mapa_shared(sm100::smem_u32(&cta_stat[rank]), 0);
+                const uint32_t dst = sm100::mapa_shared(sm100::smem_u32(&cta_stat[turn][rank]), 0);
                 if (lane < 3) {
                     const float v = lane == 0 ? st.m : lane == 1 ? st.s : st.z;
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4 * lane), "f"(v) : "memory");
                 }
                 if constexpr (TOP) {
-                    const uint32_t dk = sm100::mapa_shared(sm100::smem_u32(&cta_list[rank][lane]), 0);
-                    asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(dk), "l"(mine) : "memory");
+                    const uint32_t dk = sm100::mapa_shared(sm100::smem_u32(&cta_list[turn][rank][lane]), 0);
+                    asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(dk), "l"(best) : "memory");
                 }
             }
-            sm100::cluster_sync();
-            if (warp == 0 && rank == 0) {
-                st = cta_stat[0];
-                for (int w = 1; w < cluster; ++w) st = join(st, cta_stat[w], c);
+            __syncwarp();
+            sm100::cluster_sync();  // the other of the two buffers has been read: rank 0 came past its reads to get here
+            if (rank == 0) {
+                if (warp == 0) st = warp_join(lane < cluster ? cta_stat[turn][lane] : Stat{-INFINITY, 0.f, 0.f}, c);
                 if constexpr (TOP) {
-                    mine = cta_list[0][lane];
-                    for (int w = 1; w < cluster; ++w) mine = merge_lanes(mine, cta_list[w], lane);
+                    best = warp < cluster ? cta_list[turn][warp][lane] : 0;
+                    if (WARPS < kMaxCluster && warp + WARPS < cluster) best = merge_lanes(best, cta_list[turn][warp + WARPS], lane);
+                    best = merge_block<WARPS>(best, lists, warp, lane);
                 }
             }
         }
@@ -420,14 +487,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             if constexpr (TOP) {
                 if (lane < a.top) {
                     const bool bad = st.s != st.s;  // a NaN or +inf: no distribution
-                    const float v = from_ordered(static_cast<uint32_t>(mine >> 32));
-                    a.top_ids[r * a.top + lane] = bad ? -1 : static_cast<int>(~static_cast<uint32_t>(mine));
+                    const float v = from_ordered(static_cast<uint32_t>(best >> 32));
+                    a.top_ids[r * a.top + lane] = bad ? -1 : static_cast<int>(~static_cast<uint32_t>(best));
                     a.top_logprobs[r * a.top + lane] = bad ? NAN : empty ? -INFINITY : (v - m) * a.inv_t - log_s;
                 }
             }
         }
         __syncthreads();  // the shared arrays are reused by the next row
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- backward
@@ -450,6 +518,25 @@ struct RowGrad {
     __device__ __forceinline__ float operator()(float x, long long i) const {
         const float lp2 = max_nan((x - m) * c, kZFloor) - log2_s;
         return fmaf(ex2(lp2), fmaf(gb, lp2, ga), i == target ? gt : 0.f);
+    }
+    // the same for a chunk of elements i0, i0 + 1, ...
+    template <int E> __device__ __forceinline__ void chunk(float (&v)[E], long long i0) const {
+        const uint64_t negm = pack_f32x2(-m, -m), c2 = pack_f32x2(c, c), negs = pack_f32x2(-log2_s, -log2_s);
+        const uint64_t a2 = pack_f32x2(ga, ga), b2 = pack_f32x2(gb, gb);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            float lo, hi;
+            unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(v[e], v[e + 1]), negm), c2), lo, hi);
+            const uint64_t lp = add_f32x2(pack_f32x2(max_nan(lo, kZFloor), max_nan(hi, kZFloor)), negs);
+            unpack_f32x2(lp, lo, hi);
+            unpack_f32x2(mul_f32x2(pack_f32x2(ex2(lo), ex2(hi)), fma_f32x2(b2, lp, a2)), v[e], v[e + 1]);
+        }
+        const long long at = target - i0;
+        if (at >= 0 && at < E) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (e == at) v[e] += gt;
+        }
     }
 };
 
@@ -503,8 +590,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_grad_k
                         for (int e = 0; e < E; ++e) v[e] = 0.f;
                     } else {
                         Elems<T>::unpack(q[j], v);
-#pragma unroll
-                        for (int e = 0; e < E; ++e) v[e] = g(v[e], i0 + e);
+                        g.chunk(v, i0);
                     }
                     __stcs(dbase + cc, Elems<T>::pack(v));
                 } else {
@@ -524,31 +610,42 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_grad_k
 
 // ---------------------------------------------------------------- host side
 
-// CTAs that share a row: as many as fill the SMs once, while each still gets
-// two batches of loads per thread.
-int cluster_for(long long rows, long long chunks, int threads) {
-    int cl = 1;
-    while (cl < 8 && rows * cl * 2 <= sm_count() && chunks / (cl * 2) >= 2 * threads) cl *= 2;
-    return cl;
+// CTAs that share a row: the cluster size with the least work on the slowest
+// CTA, a row costing its share of the chunks plus about 1024 chunks' time for its
+// joins, and 128 more for each doubling of the cluster.
+int cluster_for(long long rows, long long chunks, long long slots) {
+    int best = 1;
+    double least = 0, joins = 1024;
+    for (int cl = 1; cl <= kMaxCluster; cl *= 2, joins += 128) {
+        const long long clusters = slots / cl;
+        const double cost = static_cast<double>((rows + clusters - 1) / clusters) * (static_cast<double>(chunks) / cl + joins);
+        if (cl == 1 || cost < least) {
+            least = cost;
+            best = cl;
+        }
+    }
+    return best;
 }
 
 template <typename T, int THREADS, bool TOP> int launch_forward(const LogprobArgs& a, cudaStream_t st) {
     const long long chunks = (a.vocab + Elems<T>::E - 1) / Elems<T>::E + 1;
-    const int cl = cluster_for(a.rows, chunks, THREADS);
+    const long long slots = static_cast<long long>(sm_count()) * (1024 / THREADS);
+    const int cl = cluster_for(a.rows, chunks, slots);
+    const size_t smem = sizeof(uint4) * kStages * kUnroll * THREADS;
     auto logprobs_kern = token_logprobs_kernel<T, THREADS, TOP>;
-    if (cl > 1) {
-        launch_pdl_cluster(logprobs_kern, static_cast<unsigned>(a.rows * cl), THREADS, static_cast<unsigned>(cl), 0, st, a, cl);
-    } else {
-        const long long cap = static_cast<long long>(sm_count()) * (1024 / THREADS);
-        launch_pdl(logprobs_kern, static_cast<unsigned>(a.rows < cap ? a.rows : cap), THREADS, 0, st, a, 1);
-    }
+    static SmemLimit limit;
+    if (int rc = limit.ensure(logprobs_kern, static_cast<int>(smem), "token_logprobs")) return rc;
+    const long long most = slots / cl;
+    const unsigned grid = static_cast<unsigned>((a.rows < most ? a.rows : most) * cl);
+    if (cl > 1) launch_pdl_cluster(logprobs_kern, grid, THREADS, static_cast<unsigned>(cl), smem, st, a, cl);
+    else launch_pdl(logprobs_kern, grid, THREADS, smem, st, a, 1);
     return launch_status("token_logprobs");
 }
 
 template <typename T> int forward(const LogprobArgs& a, cudaStream_t st) {
     const bool small = a.vocab <= 512 * Elems<T>::E;
-    if (a.top > 0) return small ? launch_forward<T, 128, true>(a, st) : launch_forward<T, 512, true>(a, st);
-    return small ? launch_forward<T, 128, false>(a, st) : launch_forward<T, 512, false>(a, st);
+    if (a.top > 0) return small ? launch_forward<T, 128, true>(a, st) : launch_forward<T, 256, true>(a, st);
+    return small ? launch_forward<T, 128, false>(a, st) : launch_forward<T, 256, false>(a, st);
 }
 
 template <typename T, int THREADS, bool VEC> int launch_backward(const LogprobGradArgs& a, cudaStream_t st) {
