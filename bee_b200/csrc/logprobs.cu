@@ -14,13 +14,20 @@
 // All statistics are fp32.  x - m is formed before the scaling, so that the
 // error of z does not grow with the size of the logits.
 //
-// Alternatives: a thread's running maximum is also the largest element of its
-// share of the row.  The k-th largest of these maxima bounds the row's k-th
-// largest element from below, and every element above the bound lies in the
-// share of one of the k threads with the largest maxima.  So the stream needs
-// no list of candidates: after it, k shares (of a few hundred elements each) are
-// read again from L2 and inserted into lists of 32 keys held one per lane.
-// Keys are (value, ~index) in 64 bits: ties go to the lowest index.
+// Alternatives: the stream keeps, per thread, the maxima of its two best batches
+// of chunks, which they are, and the best of the others.  The maxima of 64 groups of
+// threads (the same lane of half of the warps) give a bound: the k-th largest of them
+// is reached by an element of each of k groups, so it is at most the k-th largest
+// element, and on rows without structure only about 64 ln(64 / (64 - k)) elements
+// reach it (24 for k = 20, 44 for k = 32).  Each warp reads the batches of its threads whose
+// maxima do again (one or two of a thread, all of them if its third may), an element
+// per lane, and lists the elements that reach the bound; the rank of each among all is
+// counted.  Order is that of (value, ~index) keys of 64 bits: ties go to the lowest index.
+// Rows with more such elements than a list holds (many ties, or hardly anything
+// unmasked) insert them one by one into sorted lists instead.
+// This costs latency at the end of a row (4 rows of 131072 bf16: 4.5 us without
+// alternatives, 8.6 us with 20); sorting the group maxima and merging the warps' lists
+// took 1 to 4 us more, reading the whole shares of the threads concerned 2 to 10 us.
 //
 // Few rows: a cluster of up to 8 CTAs shares a row and joins its partial
 // results through distributed shared memory (no workspace, fixed order).
@@ -39,6 +46,9 @@ constexpr int kTopMax = 32;
 // Floor of z * log2(e): 2^-16384 is 0 in fp32, and 0 * -16384 is 0, so masked
 // (-inf) and far-off logits add nothing to S and Z; a NaN passes through.
 constexpr float kZFloor = -16384.f;
+// How far (in powers of two) a term may exceed 1 before the sums are moved to the
+// new maximum: 2^30 terms of 2^16 stay far inside fp32.
+constexpr float kSlack = 16.f;
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float d;
@@ -66,6 +76,12 @@ template <> struct Elems<float> {
     static __device__ __forceinline__ float max(uint4 q) {
         return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
     }
+    template <int N> static __device__ __forceinline__ float max(const uint4 (&q)[N]) {
+        float m = max(q[0]);
+#pragma unroll
+        for (int j = 1; j < N; ++j) m = fmaxf(m, max(q[j]));
+        return m;
+    }
     static __device__ __forceinline__ uint4 fill() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
 };
 template <> struct Elems<__nv_bfloat16> {
@@ -80,9 +96,17 @@ template <> struct Elems<__nv_bfloat16> {
         return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
     }
     static __device__ __forceinline__ __nv_bfloat162 h2(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+    static __device__ __forceinline__ __nv_bfloat162 max2(uint4 q) { return __hmax2(__hmax2(h2(q.x), h2(q.y)), __hmax2(h2(q.z), h2(q.w))); }
+    template <int N> static __device__ __forceinline__ float max(const uint4 (&q)[N]) {
+        __nv_bfloat162 m = max2(q[0]);
+#pragma unroll
+        for (int j = 1; j < N; ++j) m = __hmax2(m, max2(q[j]));
+        const float2 f = __bfloat1622float2(m);
+        return fmaxf(f.x, f.y);
+    }
     static __device__ __forceinline__ float max(uint4 q) {
-        const float2 m = __bfloat1622float2(__hmax2(__hmax2(h2(q.x), h2(q.y)), __hmax2(h2(q.z), h2(q.w))));
-        return fmaxf(m.x, m.y);
+        const float2 f = __bfloat1622float2(max2(q));
+        return fmaxf(f.x, f.y);
     }
     static __device__ __forceinline__ uint4 fill() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
 };
@@ -103,9 +127,17 @@ template <> struct Elems<__half> {
     static __device__ __forceinline__ uint4 pack(const float* v) {
         return make_uint4(pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3]), pack_f16x2(v[4], v[5]), pack_f16x2(v[6], v[7]));
     }
+    static __device__ __forceinline__ __half2 max2(uint4 q) { return __hmax2(__hmax2(h2(q.x), h2(q.y)), __hmax2(h2(q.z), h2(q.w))); }
+    template <int N> static __device__ __forceinline__ float max(const uint4 (&q)[N]) {
+        __half2 m = max2(q[0]);
+#pragma unroll
+        for (int j = 1; j < N; ++j) m = __hmax2(m, max2(q[j]));
+        const float2 f = __half22float2(m);
+        return fmaxf(f.x, f.y);
+    }
     static __device__ __forceinline__ float max(uint4 q) {
-        const float2 m = __half22float2(__hmax2(__hmax2(h2(q.x), h2(q.y)), __hmax2(h2(q.z), h2(q.w))));
-        return fmaxf(m.x, m.y);
+        const float2 f = __half22float2(max2(q));
+        return fmaxf(f.x, f.y);
     }
     static __device__ __forceinline__ uint4 fill() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
 };
@@ -146,6 +178,33 @@ struct Stat {
     float m, s, z;  // maximum, sum of 2^(z_i), sum of 2^(z_i) z_i; z_i = (x_i - m) / T * log2(e)
 };
 
+// Adds the sums of 2^z and 2^z z over a chunk, z = (x - m) c.  Where x is -inf the
+// second would be 0 * -inf = NaN; FLOOR replaces z below kZFloor by it.
+template <typename T, bool FLOOR>
+__device__ __forceinline__ void chunk_sums(uint4 q, uint64_t negm2, uint64_t c2, uint64_t& s2, uint64_t& z2) {
+    constexpr int E = Elems<T>::E;
+    float v[E];
+    Elems<T>::unpack(q, v);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+        const uint64_t d = mul_f32x2(add_f32x2(pack_f32x2(v[e], v[e + 1]), negm2), c2);
+        float lo, hi;
+        unpack_f32x2(d, lo, hi);
+        if (FLOOR) {
+            lo = max_nan(lo, kZFloor);
+            hi = max_nan(hi, kZFloor);
+        }
+        const uint64_t e2 = pack_f32x2(ex2(lo), ex2(hi));
+        s2 = add_f32x2(s2, e2);
+        z2 = fma_f32x2(e2, FLOOR ? pack_f32x2(lo, hi) : d, z2);
+    }
+}
+__device__ __forceinline__ float pair_sum(uint64_t v) {
+    float lo, hi;
+    unpack_f32x2(v, lo, hi);
+    return lo + hi;
+}
+
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Moves the sums from maximum st.m to maximum m (>= st.m).
@@ -181,39 +240,17 @@ __device__ __forceinline__ uint64_t make_key(float v, uint32_t index) {
     return (static_cast<uint64_t>(ordered(v)) << 32) | static_cast<uint32_t>(~index);
 }
 
-// One step of a bitonic network over the lanes: the lane keeps the larger key
+// One step of a bitonic merge over the lanes: the lane keeps the larger value
 // of itself and lane ^ d if `up`, else the smaller.
-__device__ __forceinline__ uint64_t exchange(uint64_t k, int d, bool up) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, k, d);
+template <typename K> __device__ __forceinline__ K exchange(K k, int d, bool up) {
+    const K o = __shfl_xor_sync(0xffffffffu, k, d);
     return ((o > k) == up) ? o : k;
 }
-// Sorts 32 keys, one per lane, largest first.
-__device__ __forceinline__ uint64_t sort_lanes(uint64_t k, int lane) {
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int d = size >> 1; d > 0; d >>= 1) k = exchange(k, d, ((lane & d) == 0) == ((lane & size) == 0));
-    return k;
-}
-// The 32 largest of two lists sorted largest first (keys are distinct, or 0).
-__device__ __forceinline__ uint64_t merge_lanes(uint64_t k, const uint64_t* other, int lane) {
-    const uint64_t o = other[31 - lane];
-    k = o > k ? o : k;
+// The 32 largest of a list sorted largest first and `other`, the other list's value at 31 - lane.
+template <typename K> __device__ __forceinline__ K merge_lanes(K k, K other, int lane) {
+    k = other > k ? other : k;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) k = exchange(k, d, (lane & d) == 0);
-    return k;
-}
-
-// The 32 largest keys of the block's warps' sorted lists, in warp 0 (others: undefined).
-template <int WARPS>
-__device__ __forceinline__ uint64_t merge_block(uint64_t k, uint64_t (*lists)[32], int warp, int lane) {
-#pragma unroll
-    for (int half = WARPS / 2; half > 0; half >>= 1) {
-        if (warp >= half && warp < 2 * half) lists[warp][lane] = k;
-        __syncthreads();
-        if (warp < half) k = merge_lanes(k, lists[warp + half], lane);
-        __syncthreads();
-    }
     return k;
 }
 
@@ -238,8 +275,14 @@ constexpr int kUnroll = 4;  // chunks of a thread per batch
 constexpr int kMaxCluster = 8;
 constexpr int kStages = 3;  // batches in its part of the shared-memory ring
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(dst)), "l"(src) : "memory");
+// 16 bytes from global to shared memory, both addresses moved by OFF bytes.
+template <int OFF> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %2], 16;" ::"r"(dst), "l"(src), "n"(OFF) : "memory");
+}
+template <int OFF> __device__ __forceinline__ uint4 lds16(uint32_t src) {
+    uint4 q;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(src), "n"(OFF) : "memory");
+    return q;
 }
 
 // One CTA's part of a row: the whole chunks [lo, hi) and perhaps the partial
@@ -255,10 +298,6 @@ template <typename T> struct Part {
         edge_lo = rank == 0 && row.full_lo > 0 ? 0 : -1;
         edge_hi = rank == cluster - 1 && row.full_hi < row.chunks && row.full_hi >= row.full_lo ? row.full_hi : -1;
     }
-    // the thread that reads chunk c
-    template <int THREADS> __device__ __forceinline__ int owner(int c) const {
-        return c == edge_lo ? 0 : c == edge_hi ? 1 : (c - lo) % THREADS;
-    }
 };
 
 // Clusters of `cluster` CTAs (1: single CTAs) take rows in grid-stride order.
@@ -268,14 +307,17 @@ template <typename T> struct Part {
 template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobArgs a, int cluster) {
     constexpr int WARPS = THREADS / 32;
-    static_assert(2 * WARPS >= kMaxCluster, "a warp of rank 0 joins at most two of the cluster's lists");
     constexpr int E = Elems<T>::E;
-    extern __shared__ __align__(16) uint4 ring[];  // [kStages][kUnroll][THREADS]
+    extern __shared__ __align__(16) uint4 ring[];  // [kStages][kUnroll][THREADS]; four CTAs of 256 threads leave 8 KiB each for the rest
     __shared__ Stat warp_stat[WARPS];
-    __shared__ Stat cta_stat[2][kMaxCluster];                // rank 0's copy is filled by the whole cluster, alternating by row
-    __shared__ uint64_t lists[WARPS][32];
-    __shared__ uint64_t cta_list[2][TOP ? kMaxCluster : 1][32];
-    __shared__ uint64_t owners[32];
+    __shared__ Stat cta_stat[kMaxCluster];  // rank 0's copy is filled by the whole cluster
+    // 7.5 KiB for the alternatives: four CTAs of 256 threads and their rings fill an SM's shared memory
+    __shared__ uint64_t lists[TOP ? WARPS : 1][32];  // each warp's elements that reach the bound
+    __shared__ int listed[WARPS];
+    __shared__ uint64_t sorted[TOP ? 32 : 1];
+    __shared__ uint64_t cta_list[TOP ? kMaxCluster : 1][32];
+    __shared__ __align__(16) float group_max[TOP ? 64 : 4];
+    __shared__ float lane_max[TOP ? WARPS : 1][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = cluster > 1 ? static_cast<int>(sm100::cluster_ctarank()) : 0;
     const float c = a.inv_t * kLog2e;
@@ -283,195 +325,307 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     pdl_wait();
     const long long step = gridDim.x / cluster, r0 = blockIdx.x / cluster;
 
-    // the batch to copy next: the issue_at-th chunk of issue_row's part onwards
+    static_assert(kUnroll == 4, "the four chunks of a batch are written out");
+    constexpr int STEP = THREADS * 16, SLOT = kUnroll * STEP;  // bytes between a thread's chunks; a slot of the ring
+    const uint32_t ring_lo = sm100::smem_u32(ring) + tid * 16, ring_hi = ring_lo + kStages * SLOT;
+    // the batch to copy next: this thread's first chunk of it, the whole batches and chunks left in the part, its slot
     long long issue_row = r0;
-    int issue_at = tid, issue_hi = 0, issue_slot = 0;
-    const uint4* issue_base = nullptr;
-    int issue_end = 0;  // uniform: batches left in the row
+    const uint4* issue_from = nullptr;
+    int issue_whole = 0, issue_rest = 0;
+    uint32_t issue_to = ring_lo;
     auto open_row = [&] {
         if (issue_row >= a.rows) return;
         const Part<T> p(a, issue_row, rank, cluster);
-        issue_base = p.row.base;
-        issue_at = p.lo + tid;
-        issue_hi = p.hi;
-        issue_end = (p.hi - p.lo + kUnroll * THREADS - 1) / (kUnroll * THREADS);
+        issue_from = p.row.base + p.lo + tid;
+        issue_whole = (p.hi - p.lo) / (kUnroll * THREADS);
+        issue_rest = (p.hi - p.lo) % (kUnroll * THREADS);
     };
     auto issue = [&] {
-        while (issue_row < a.rows && issue_end == 0) {  // rows without whole chunks have no batches
+        if (issue_whole > 0) {
+            cp_async16<0>(issue_to, issue_from);
+            cp_async16<STEP>(issue_to, issue_from);
+            cp_async16<2 * STEP>(issue_to, issue_from);
+            cp_async16<3 * STEP>(issue_to, issue_from);
+            issue_from += kUnroll * THREADS;
+            --issue_whole;
+        } else if (issue_rest > 0) {
+            const int left = issue_rest - tid;
+            if (left > 0) cp_async16<0>(issue_to, issue_from);
+            if (left > THREADS) cp_async16<STEP>(issue_to, issue_from);
+            if (left > 2 * THREADS) cp_async16<2 * STEP>(issue_to, issue_from);
+            if (left > 3 * THREADS) cp_async16<3 * STEP>(issue_to, issue_from);
+            issue_rest = 0;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");  // empty past the end: the wait counts stay uniform
+        issue_to = issue_to + SLOT == ring_hi ? ring_lo : issue_to + SLOT;
+        while (issue_whole == 0 && issue_rest == 0 && issue_row < a.rows) {  // on to the next row that has whole chunks
             issue_row += step;
             open_row();
         }
-        if (issue_row < a.rows) {
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j)
-                if (issue_at + j * THREADS < issue_hi)
-                    cp_async16(ring + (issue_slot * kUnroll + j) * THREADS + tid, issue_base + issue_at + j * THREADS);
-            issue_at += kUnroll * THREADS;
-            --issue_end;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");  // empty past the end: the wait counts stay uniform
-        issue_slot = issue_slot + 1 == kStages ? 0 : issue_slot + 1;
     };
     open_row();
+    while (issue_whole == 0 && issue_rest == 0 && issue_row < a.rows) {
+        issue_row += step;
+        open_row();
+    }
     for (int j = 1; j < kStages; ++j) issue();
 
-    int slot = 0, turn = 0;
-    for (long long r = r0; r < a.rows; r += step, turn ^= 1) {
+    uint32_t slot = ring_lo;
+    // targets are read a row ahead, by the thread that writes the row's results, so that nothing waits for them
+    const bool writer = tid == 0 && rank == 0 && a.logprob;
+    long long next_target = writer && r0 < a.rows ? target_of(a.targets, a.targets_i64, r0) : -1;
+    for (long long r = r0; r < a.rows; r += step) {
         if (r + step >= a.rows) pdl_trigger();  // this CTA's last row
         const Part<T> part(a, r, rank, cluster);
         const RowChunks<T>& row = part.row;
 
-        // early loads: the target's logit (by the thread that writes the row's results) and the partial chunks
-        long long target = -1;
-        float xt = -INFINITY;
-        if (tid == 0 && rank == 0 && a.logprob) {
-            target = target_of(a.targets, a.targets_i64, r);
+        // early loads: the target's logit and the partial chunks
+        const long long target = next_target;
+        float xt = 0.f;
+        if (writer) {
             xt = target < 0 ? 0.f : target < a.vocab ? Elems<T>::get(row.row + target) : NAN;
+            if (r + step < a.rows) next_target = target_of(a.targets, a.targets_i64, r + step);
         }
         const int edge = tid == 0 ? part.edge_lo : tid == 1 ? part.edge_hi : -1;
         uint4 edge_chunk = Elems<T>::fill();
         if (edge >= 0) edge_chunk = row.partial(edge);
 
-        Stat st{-INFINITY, 0.f, 0.f};
-        int at = -1;  // the chunk that holds this thread's maximum
-        auto consume = [&](const uint4 (&q)[kUnroll], int c0, int count) {
-            float cm[kUnroll], bm = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                cm[j] = Elems<T>::max(q[j]);
-                bm = fmaxf(bm, cm[j]);
+        Stat st{-INFINITY, 0.f, 0.f};  // st.m: a reference, at most kSlack below the maximum, so that it seldom moves
+        // the maximum; TOP: also those of this thread's two best batches, their numbers, and the best of the rest
+        float top = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+        int b1 = 0, b2 = 0;
+        bool floored = false;  // this thread has met logits so low that z or 2^z z overflows
+        auto consume = [&](uint4 (&q)[kUnroll], int b) {  // b: the batch's number, -1 for the partial chunks
+            const float bm = Elems<T>::max(q);
+            top = fmaxf(top, bm);
+            if (TOP && b >= 0) {
+                const bool first = bm > m1, second = bm > m2;
+                m3 = second ? m2 : fmaxf(m3, bm);
+                m2 = first ? m1 : second ? bm : m2;
+                b2 = first ? b1 : second ? b : b2;
+                m1 = first ? bm : m1;
+                b1 = first ? b : b1;
             }
-            // the partial first chunk comes last but holds the lowest indices: it wins a tie
-            if (bm > st.m || at < 0 || (TOP && c0 == part.edge_lo && bm == st.m)) {
-                rebase(st, bm, c);
-                at = c0;
-                if (TOP) {
-#pragma unroll
-                    for (int j = kUnroll - 1; j >= 0; --j)
-                        if (j < count && cm[j] == bm) at = c0 + j * THREADS;
-                }
-            }
+            if ((bm - st.m) * c > kSlack) rebase(st, bm, c);
             const float m = finite_max(st.m);
             const uint64_t negm2 = pack_f32x2(-m, -m), c2 = pack_f32x2(c, c);
             uint64_t s2 = 0, z2 = 0;  // pairs of fp32 zeros
+            if (!floored) {
 #pragma unroll
-            for (int j = 0; j < kUnroll; ++j) {
-                float v[E];
-                Elems<T>::unpack(q[j], v);
-#pragma unroll
-                for (int e = 0; e < E; e += 2) {
-                    float lo, hi;
-                    unpack_f32x2(mul_f32x2(add_f32x2(pack_f32x2(v[e], v[e + 1]), negm2), c2), lo, hi);
-                    lo = max_nan(lo, kZFloor);
-                    hi = max_nan(hi, kZFloor);
-                    const uint64_t e2 = pack_f32x2(ex2(lo), ex2(hi));
-                    s2 = add_f32x2(s2, e2);
-                    z2 = fma_f32x2(e2, pack_f32x2(lo, hi), z2);
+                for (int j = 0; j < kUnroll; ++j) chunk_sums<T, false>(q[j], negm2, c2, s2, z2);
+                floored = pair_sum(z2) != pair_sum(z2);
+            }
+            if (floored) {  // -inf, or a NaN
+                s2 = z2 = 0;
+#pragma unroll 1
+                for (int j = 0; j < kUnroll; ++j) {
+                    chunk_sums<T, true>(q[0], negm2, c2, s2, z2);
+                    q[0] = q[1];
+                    q[1] = q[2];
+                    q[2] = q[3];
                 }
             }
-            float lo, hi;
-            unpack_f32x2(s2, lo, hi);
-            st.s += lo + hi;
-            unpack_f32x2(z2, lo, hi);
-            st.z += lo + hi;
+            st.s += pair_sum(s2);
+            st.z += pair_sum(z2);
         };
-        for (int c0 = part.lo; c0 < part.hi; c0 += kUnroll * THREADS) {
+        // whole batches, then one for the chunks that are left, then the row's partial chunks
+        const int whole = (part.hi - part.lo) / (kUnroll * THREADS), rest = (part.hi - part.lo) % (kUnroll * THREADS);
+        const uint4 none = Elems<T>::fill();
+        for (int b = 0; b < whole; ++b) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             issue();
-            const uint4* mine = ring + slot * kUnroll * THREADS + tid;
-            slot = slot + 1 == kStages ? 0 : slot + 1;
-            const int left = part.hi - c0 - tid;  // this thread's chunks are those at 0, THREADS, ... below `left`
-            if (left <= 0) continue;
-            uint4 q[kUnroll];
-            if (left > (kUnroll - 1) * THREADS) {
-#pragma unroll
-                for (int j = 0; j < kUnroll; ++j) q[j] = mine[j * THREADS];
-                consume(q, c0 + tid, kUnroll);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kUnroll; ++j) q[j] = j * THREADS < left ? mine[j * THREADS] : Elems<T>::fill();
-                consume(q, c0 + tid, (left + THREADS - 1) / THREADS);
+            uint4 q[kUnroll] = {lds16<0>(slot), lds16<STEP>(slot), lds16<2 * STEP>(slot), lds16<3 * STEP>(slot)};
+            slot = slot + SLOT == ring_hi ? ring_lo : slot + SLOT;
+            consume(q, b);
+        }
+        if (rest > 0) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            issue();
+            const int left = rest - tid;  // this thread's chunks are those at 0, THREADS, ... below it
+            if (left > 0) {
+                uint4 q[kUnroll] = {lds16<0>(slot), left > THREADS ? lds16<STEP>(slot) : none,
+                                    left > 2 * THREADS ? lds16<2 * STEP>(slot) : none, left > 3 * THREADS ? lds16<3 * STEP>(slot) : none};
+                consume(q, whole);
             }
+            slot = slot + SLOT == ring_hi ? ring_lo : slot + SLOT;
         }
         if (edge >= 0) {
-            uint4 q[kUnroll];
-            q[0] = edge_chunk;
-#pragma unroll
-            for (int j = 1; j < kUnroll; ++j) q[j] = Elems<T>::fill();
-            consume(q, edge, 1);
+            uint4 q[kUnroll] = {edge_chunk, none, none, none};
+            consume(q, -1);
         }
         __syncwarp();
 
-        uint64_t best = 0;
         if constexpr (TOP) {
-            // owners of the k largest thread maxima
-            uint64_t key = at >= 0 ? make_key(st.m, static_cast<uint32_t>(at)) : 0;
-            key = merge_block<WARPS>(sort_lanes(key, lane), lists, warp, lane);
-            if (warp == 0) owners[lane] = key;
+            lane_max[warp][lane] = top;
+            if (tid < 32) sorted[tid] = 0;
             __syncthreads();
-            const uint32_t bound = static_cast<uint32_t>(owners[a.top - 1] >> 32);  // 0 if fewer threads hold anything
-            // inserts the elements of each lane's chunk (index cc; none where !in) into the warp's sorted list
-            auto insert = [&](uint4 chunk, int cc, bool in) {
-                float v[E];
-                Elems<T>::unpack(chunk, v);
-                const long long i0 = row.first(cc);
+            // the bound: the smallest group maximum that fewer than k others exceed (every warp finds it for itself;
+            // all of them write the same 64 maxima)
+            float g0 = lane_max[0][lane], g1 = lane_max[WARPS / 2][lane];
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const bool real = in && i0 + e >= 0 && i0 + e < row.n && v[e] == v[e] && ordered(v[e]) >= bound;
-                    if (!__any_sync(0xffffffffu, real)) continue;
-                    const uint64_t ck = real ? make_key(v[e], static_cast<uint32_t>(i0 + e)) : 0;
-                    uint32_t todo = __ballot_sync(0xffffffffu, ck > __shfl_sync(0xffffffffu, best, 31));
-                    while (todo) {
-                        const int src = __ffs(todo) - 1;
-                        todo &= todo - 1;
-                        const uint64_t nk = __shfl_sync(0xffffffffu, ck, src);
-                        const int pos = __popc(__ballot_sync(0xffffffffu, best > nk));
-                        const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
-                        best = lane < pos ? best : lane == pos ? nk : up;
-                    }
-                }
+            for (int w = 1; w < WARPS / 2; ++w) {
+                g0 = fmaxf(g0, lane_max[w][lane]);
+                g1 = fmaxf(g1, lane_max[WARPS / 2 + w][lane]);
+            }
+            group_max[lane] = g0;
+            group_max[32 + lane] = g1;
+            __syncwarp();
+            int n0 = 0, n1 = 0;
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const float4 g = reinterpret_cast<const float4*>(group_max)[i];
+                n0 += (g.x > g0) + (g.y > g0) + (g.z > g0) + (g.w > g0);
+                n1 += (g.x > g1) + (g.y > g1) + (g.z > g1) + (g.w > g1);
+            }
+            const uint32_t o0 = n0 < a.top ? ordered(g0) : 0xffffffffu, o1 = n1 < a.top ? ordered(g1) : 0xffffffffu;
+            const float bound = from_ordered(__reduce_min_sync(0xffffffffu, o0 < o1 ? o0 : o1));
+
+            // the warp's elements that reach it
+            const int batches = whole + (rest > 0);
+            int held = 0;
+            auto list = [&](float x, long long i) {  // an element per lane, NaN for none
+                const uint32_t hit = __ballot_sync(0xffffffffu, x >= bound);
+                const int at = held + __popc(hit & ((1u << lane) - 1u));
+                if (x >= bound && at < 32) lists[warp][at] = make_key(x, static_cast<uint32_t>(i));
+                held += __popc(hit);
             };
-            for (int j = warp; j < a.top; j += WARPS) {
-                const uint64_t o = owners[j];
-                if (o == 0) break;  // the list is sorted: no more owners
-                const int owner = part.template owner<THREADS>(static_cast<int>(~static_cast<uint32_t>(o)));
-                for (int cb = part.lo + owner; cb < part.hi; cb += 32 * THREADS) {
-                    const int cc = cb + lane * THREADS;
-                    insert(cc < part.hi ? __ldg(row.base + cc) : Elems<T>::fill(), cc, cc < part.hi);
+            const bool every = m3 >= bound;  // more than two of this thread's batches may reach it
+            int b = every ? 0 : b1, todo = every ? batches : static_cast<int>(m1 >= bound) + static_cast<int>(m2 >= bound);
+            constexpr int AHEAD = 4;  // batches whose loads are in flight together
+            const int chunk = lane / E;  // this lane's element of a batch: element lane % E of its owner's chunk lane / E
+#pragma unroll 1
+            for (uint32_t left = __ballot_sync(0xffffffffu, todo > 0); left != 0 && held <= 32; left = __ballot_sync(0xffffffffu, todo > 0)) {
+                const int mine = part.lo + b * kUnroll * THREADS + tid;
+                float x[AHEAD];
+                long long at[AHEAD];
+                uint32_t now = left;
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int from = now ? __ffs(now) - 1 : 0;
+                    const int cc = __shfl_sync(0xffffffffu, mine, from) + chunk * THREADS;
+                    at[i] = row.first(cc) + lane % E;
+                    x[i] = now != 0 && chunk < kUnroll && cc < part.hi ? Elems<T>::get(row.row + at[i]) : NAN;
+                    now &= now - 1;  // 0 stays 0
                 }
-                const int partial = owner == 0 ? part.edge_lo : owner == 1 ? part.edge_hi : -1;
-                if (partial >= 0) insert(lane == 0 ? row.partial(partial) : Elems<T>::fill(), partial, lane == 0);
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) list(x[i], at[i]);
+                if ((left & ~now) >> lane & 1u) {
+                    --todo;
+                    b = every ? b + 1 : b2;
+                }
+            }
+            if (warp == 0) {  // the partial chunks
+                float x[2] = {NAN, NAN};
+                long long at[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = i == 0 ? part.edge_lo : part.edge_hi;
+                    at[i] = row.first(e) + lane;
+                    if (e >= 0 && lane < E && at[i] >= 0 && at[i] < row.n) x[i] = Elems<T>::get(row.row + at[i]);
+                }
+                list(x[0], at[0]);
+                list(x[1], at[1]);
+            }
+            if (lane == 0) listed[warp] = held;
+            __syncthreads();
+            bool over = false;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) over |= listed[w] > 32;
+            if (!over) {
+                if (lane < held) {
+                    const uint64_t key = lists[warp][lane];
+                    int place = 0;
+#pragma unroll 1
+                    for (int w = 0; w < WARPS; ++w) {
+                        const int n = listed[w];
+#pragma unroll 4
+                        for (int i = 0; i < n; ++i) place += lists[w][i] > key;
+                    }
+                    if (place < a.top) sorted[place] = key;
+                }
+            } else {
+                // inserts the elements of each lane's chunk (index cc, none where !in) that reach the bound into the
+                // warp's sorted list: chunk by chunk, its elements spread over the lanes
+                uint64_t best = 0;
+                auto insert = [&](uint4 q0, int cc, bool in) {
+                    const float cm = Elems<T>::max(q0);
+                    // no key of the chunk is larger than this one
+                    const uint64_t most = in && cm >= bound ? make_key(cm, static_cast<uint32_t>(max(row.first(cc), 0ll))) : 0;
+                    uint32_t hits = __ballot_sync(0xffffffffu, most > __shfl_sync(0xffffffffu, best, a.top - 1));
+#pragma unroll 1
+                    while (hits) {
+                        const int from = __ffs(hits) - 1;
+                        hits &= hits - 1;
+                        if (__shfl_sync(0xffffffffu, most, from) <= __shfl_sync(0xffffffffu, best, a.top - 1)) continue;
+                        const long long i = row.first(__shfl_sync(0xffffffffu, cc, from)) + lane;
+                        const float x = lane < E && i >= 0 && i < row.n ? Elems<T>::get(row.row + i) : NAN;
+                        const uint64_t ck = x >= bound ? make_key(x, static_cast<uint32_t>(i)) : 0;
+                        uint32_t more = __ballot_sync(0xffffffffu, ck > __shfl_sync(0xffffffffu, best, a.top - 1));
+#pragma unroll 1
+                        while (more) {
+                            const int src = __ffs(more) - 1;
+                            more &= more - 1;
+                            const uint64_t nk = __shfl_sync(0xffffffffu, ck, src);
+                            const int pos = __popc(__ballot_sync(0xffffffffu, best > nk));
+                            const uint64_t up = __shfl_up_sync(0xffffffffu, best, 1);
+                            best = lane < pos ? best : lane == pos ? nk : up;
+                        }
+                    }
+                };
+#pragma unroll 1
+                for (int cb = part.lo + warp * 32; cb < part.hi; cb += THREADS) {
+                    const int cc = cb + lane;
+                    insert(cc < part.hi ? __ldg(row.base + cc) : none, cc, cc < part.hi);
+                }
+                insert(edge_chunk, edge, edge >= 0);
+                __syncthreads();  // the lists above are no longer read
+                lists[warp][lane] = best;
+                __syncthreads();
+                if (warp == 0) {
+#pragma unroll 1
+                    for (int w = 1; w < WARPS; ++w) best = merge_lanes(best, lists[w][31 - lane], lane);
+                    if (lane < a.top) sorted[lane] = best;
+                }
             }
         }
 
         // join the block's statistics, then the cluster's, each in a fixed order
+        rebase(st, top, c);
         st = warp_join(st, c);
         if (lane == 0) warp_stat[warp] = st;
-        if constexpr (TOP) best = merge_block<WARPS>(best, lists, warp, lane);
         __syncthreads();
-        if (warp == 0) st = warp_join(lane < WARPS ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f}, c);
+        uint64_t best = 0;  // TOP, warp 0: key of this lane's alternative
+        if (warp == 0) {
+            st = warp_join(lane < WARPS ? warp_stat[lane] : Stat{-INFINITY, 0.f, 0.f}, c);
+            if (TOP) best = sorted[lane];
+        }
         if (cluster > 1) {
             if (warp == 0) {
-                const uint32_t dst = sm100::mapa_shared(sm100::smem_u32(&cta_stat[turn][rank]), 0);
+                const uint32_t dst = sm100::mapa_shared(sm100::smem_u32(&cta_stat[rank]), 0);
                 if (lane < 3) {
                     const float v = lane == 0 ? st.m : lane == 1 ? st.s : st.z;
                     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + 4 * lane), "f"(v) : "memory");
                 }
                 if constexpr (TOP) {
-                    const uint32_t dk = sm100::mapa_shared(sm100::smem_u32(&cta_list[turn][rank][lane]), 0);
+                    const uint32_t dk = sm100::mapa_shared(sm100::smem_u32(&cta_list[rank][lane]), 0);
                     asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(dk), "l"(best) : "memory");
                 }
             }
             __syncwarp();
-            sm100::cluster_sync();  // the other of the two buffers has been read: rank 0 came past its reads to get here
+            sm100::cluster_sync();
             if (rank == 0) {
-                if (warp == 0) st = warp_join(lane < cluster ? cta_stat[turn][lane] : Stat{-INFINITY, 0.f, 0.f}, c);
+                if (warp == 0) st = warp_join(lane < cluster ? cta_stat[lane] : Stat{-INFINITY, 0.f, 0.f}, c);
                 if constexpr (TOP) {
-                    best = warp < cluster ? cta_list[turn][warp][lane] : 0;
-                    if (WARPS < kMaxCluster && warp + WARPS < cluster) best = merge_lanes(best, cta_list[turn][warp + WARPS], lane);
-                    best = merge_block<WARPS>(best, lists, warp, lane);
+#pragma unroll 1
+                    for (int half = cluster / 2; half > 0; half >>= 1) {  // a tree over the CTAs' lists, a warp per pair
+                        if (warp < half)
+                            cta_list[warp][lane] = merge_lanes(cta_list[warp][lane], cta_list[warp + half][31 - lane], lane);
+                        __syncthreads();
+                    }
+                    best = cta_list[0][lane];
                 }
             }
+            if (r + step < a.rows) sm100::cluster_sync();  // rank 0 has read the partial results: the next row's may come
         }
         if (warp == 0 && rank == 0) {
             const bool empty = st.m == -INFINITY && st.s == 0.f;
