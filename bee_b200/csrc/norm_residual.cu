@@ -115,9 +115,48 @@ template <typename T, bool VEC, int THREADS> struct Cols {
             return make_uint4(Conv<T>::down2(v[0]), Conv<T>::down2(v[1]), Conv<T>::down2(v[2]), Conv<T>::down2(v[3]));
         }
     }
+    // bytes of a row in a ring slot
+    static constexpr bool kPadded = VEC && THREADS < 1024;  // slots as wide as the block's columns, zero past the row's end
+    static __host__ __device__ constexpr uint32_t pitch(uint32_t cols) {
+        return kPadded ? THREADS * kEpt * sizeof(T) : (cols * static_cast<uint32_t>(sizeof(T)) + 15) / 16 * 16 + (VEC ? 0 : 16);
+    }
+    // zeros where this thread's vectors of a slot lie past the row's end
+    __device__ __forceinline__ void pad(uint8_t* slot) const {
+        if constexpr (kPadded) {
+#pragma unroll
+            for (int j = 0; j < kEpt / E; ++j)
+                if (vec(j) * E >= cols) reinterpret_cast<uint4*>(slot)[vec(j)] = make_uint4(0, 0, 0, 0);
+        }
+    }
+    // this thread's columns of an optional vector into a slot (absent: ones), which only this thread reads
+    __device__ __forceinline__ void keep(T* slot, const T* w) const {
+        f2 v[kPairs];
+        if (w) {
+            read<true>(w, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = dup(1.f);
+        }
+        if constexpr (VEC) {
+#pragma unroll
+            for (int j = 0; j < kEpt / E; ++j)
+                if (kPadded || vec(j) * E < cols) reinterpret_cast<uint4*>(slot)[vec(j)] = pack(v + j * (E / 2));
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                float a, b;
+                unpack_f32x2(v[k], a, b);
+                if (col(2 * k) < cols) slot[col(2 * k)] = Conv<T>::down(a);
+                if (col(2 * k + 1) < cols) slot[col(2 * k + 1)] = Conv<T>::down(b);
+            }
+        }
+    }
     // from a row (shared or global memory; LDG: read-only global vectors)
     template <bool LDG> __device__ __forceinline__ void read(const T* p, f2 (&v)[kPairs]) const {
-        if constexpr (VEC) {
+        if constexpr (kPadded && !LDG) {
+#pragma unroll
+            for (int j = 0; j < kEpt / E; ++j) unpack(reinterpret_cast<const uint4*>(p)[vec(j)], v + j * (E / 2));
+        } else if constexpr (VEC) {
 #pragma unroll
             for (int j = 0; j < kEpt / E; ++j) {
                 const uint4* q = reinterpret_cast<const uint4*>(p) + vec(j);
@@ -154,16 +193,25 @@ template <typename T, bool VEC, int THREADS> struct Cols {
             }
         }
     }
-    // fp32 partial sums, in this thread's own order (any fixed place per column would do)
+    // fp32 partial sums (p 16-byte aligned)
     __device__ __forceinline__ void write_f32(float* p, const f2 (&v)[kPairs]) const {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) {
-            float a, b;
-            unpack_f32x2(v[k], a, b);
-            const uint32_t ca = VEC ? vec(2 * k / E) * E + 2 * k % E : col(2 * k);
-            const uint32_t cb = VEC ? ca + 1 : col(2 * k + 1);
-            if (ca < cols) p[ca] = a;
-            if (cb < cols) p[cb] = b;
+            for (int k = 0; k < kPairs; k += 2) {
+                const uint32_t c = vec(2 * k / E) * E + 2 * k % E;
+                float4 q;
+                unpack_f32x2(v[k], q.x, q.y);
+                unpack_f32x2(v[k + 1], q.z, q.w);
+                if (c < cols) *reinterpret_cast<float4*>(p + c) = q;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                float a, b;
+                unpack_f32x2(v[k], a, b);
+                if (col(2 * k) < cols) p[col(2 * k)] = a;
+                if (col(2 * k + 1) < cols) p[col(2 * k + 1)] = b;
+            }
         }
     }
     __device__ __forceinline__ void read_f32(const float* p, f2 (&v)[kPairs]) const {
@@ -179,23 +227,41 @@ template <typename T, bool VEC, int THREADS> struct Cols {
 // Sums over the block with one barrier: consecutive calls use alternating halves
 // of `red`, so a call's writes never meet the previous call's reads.
 template <int THREADS> struct BlockSum {
-    float2 (*red)[THREADS / 32];
+    static constexpr int WARPS = THREADS / 32;
+    f2 (*red)[WARPS];  // a warp's two sums, or one
     int parity = 0;
+    // of a and b, at once
     __device__ __forceinline__ float2 operator()(float a, float b) {
         a = warp_sum(a);
         b = warp_sum(b);
         if constexpr (THREADS == 32) return make_float2(a, b);
-        if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = make_float2(a, b);
+        if ((threadIdx.x & 31) == 0) red[parity][threadIdx.x >> 5] = pack_f32x2(a, b);
         __syncthreads();
-        float2 r = make_float2(0.f, 0.f);
+        f2 r = 0;
 #pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            const float2 v = red[parity][w];
-            r.x += v.x;
-            r.y += v.y;
+        for (int w = 0; w < WARPS; w += 2) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&red[parity][w]);
+            r = add_f32x2(add_f32x2(r, v.x), v.y);
         }
         parity ^= 1;
-        return r;
+        float2 s;
+        unpack_f32x2(r, s.x, s.y);
+        return s;
+    }
+    __device__ __forceinline__ float operator()(float a) {
+        a = warp_sum(a);
+        if constexpr (THREADS == 32) return a;
+        float* one = reinterpret_cast<float*>(red[parity]);
+        if ((threadIdx.x & 31) == 0) one[threadIdx.x >> 5] = a;
+        __syncthreads();
+        f2 r = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; w += 4) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(one + w);
+            r = add_f32x2(add_f32x2(r, v.x), v.y);
+        }
+        parity ^= 1;
+        return hsum(r);
     }
 };
 
@@ -262,7 +328,9 @@ template <typename T, bool VEC, int THREADS, int NT> struct Ring {
             issue();
         }
     }
-    __device__ __forceinline__ void start() {
+    template <typename C> __device__ __forceinline__ void start(const C& cl) {
+        for (uint32_t s = 0; s < stages; ++s)
+            for (int t = 0; t < NT; ++t) cl.pad(at(s, t));
         for (uint32_t s = 1; s < stages; ++s) issue();
     }
 };
@@ -272,9 +340,9 @@ struct NormArgs {
     void *x_out, *y;
     const void *dx_out, *dy;
     void *dh, *dx, *dgate;
-    float *part_post, *part_pre, *part_gate;  // partial sums: [ctas][cols], [ctas][cols], [2 * ctas][cols]
+    float *part_post, *part_pre, *part_gate;  // partial sums: [ctas][part], [ctas][part], [2 * ctas][part]
     long long rows, per_cta, group;           // group: rows per gate row
-    uint32_t cols, pitch, stages;
+    uint32_t cols, part, pitch, stages;       // part: cols rounded up to 4
     float alpha, beta, eps;
 };
 
@@ -283,7 +351,7 @@ struct NormArgs {
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ float2 red[2][THREADS / 32];
+    __shared__ __align__(16) f2 red[2][THREADS / 32];
     BlockSum<THREADS> block_sum{red};
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
@@ -292,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
     const float inv_n = 1.0f / static_cast<float>(a.cols);
     Ring<T, VEC, THREADS, 2> ring{{static_cast<const T*>(a.h), static_cast<const T*>(a.x)}, ring_smem, a.cols, a.pitch, a.stages, r0, r1};
     pdl_wait();
-    ring.start();
+    ring.start(cl);
     uint32_t slot = 0;
     for (long long r = r0; r < r1; ++r, slot = slot + 1 == a.stages ? 0 : slot + 1) {
         if (r + 1 >= r1) pdl_trigger();
@@ -304,7 +372,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
             f2 ss = 0;
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(v[k], v[k], ss);
-            scale *= rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps));
+            scale *= rsqrtf(fmaf(block_sum(hsum(ss)), inv_n, a.eps));
             cl.weights(wpost, t);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], t[k]);
@@ -323,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
         }
         cl.write(static_cast<T*>(a.x_out) + r * a.cols, v);
         if (wpre) {
-            const f2 rx = dup(rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps)));
+            const f2 rx = dup(rsqrtf(fmaf(block_sum(hsum(ss)), inv_n, a.eps)));
             cl.weights(wpre, t);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(mul_f32x2(v[k], rx), t[k]);
@@ -340,7 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
 template <typename T, bool VEC, int THREADS, bool REG>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ float2 red[2][THREADS / 32];
+    __shared__ __align__(16) f2 red[2][THREADS / 32];
     BlockSum<THREADS> block_sum{red};
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
@@ -350,21 +418,34 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
     const float inv_n = 1.0f / static_cast<float>(a.cols);
     Ring<T, VEC, THREADS, 4> ring{{static_cast<const T*>(a.h), static_cast<const T*>(a.x), static_cast<const T*>(a.dx_out),
                                    static_cast<const T*>(a.dy)}, ring_smem, a.cols, a.pitch, a.stages, r0, r1};
-    float* my_post = a.part_post + static_cast<long long>(blockIdx.x) * a.cols;
-    float* my_pre = a.part_pre + static_cast<long long>(blockIdx.x) * a.cols;
-    float* my_gate = a.part_gate + static_cast<long long>(blockIdx.x) * 2 * a.cols;
+    float* my_post = a.part_post + static_cast<long long>(blockIdx.x) * a.part;
+    float* my_pre = a.part_pre + static_cast<long long>(blockIdx.x) * a.part;
+    float* my_gate = a.part_gate + static_cast<long long>(blockIdx.x) * 2 * a.part;
     f2 s_post[kPairs], s_pre[kPairs], s_gate[kPairs];
 #pragma unroll
     for (int k = 0; k < kPairs; ++k) s_post[k] = s_pre[k] = s_gate[k] = 0;
+    // the three vectors follow the ring, each thread's own columns (REG)
+    T* keep_post = reinterpret_cast<T*>(ring_smem + a.pitch * 4 * a.stages);
+    T* keep_pre = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 1));
+    T* keep_gate = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 2));
     pdl_wait();
-    ring.start();
+    ring.start(cl);
+    if constexpr (REG) {
+        cl.keep(keep_post, wpost);
+        cl.keep(keep_pre, wpre);
+        cl.keep(keep_gate, gate ? gate + r0 / a.group * a.cols : nullptr);
+    }
+    // a vector's columns, from there or (rows too wide for that) from global memory
+    auto vector = [&](const T* kept, const T* global, f2 (&out)[kPairs]) {
+        if constexpr (REG) cl.template read<false>(kept, out);
+        else cl.weights(global, out);
+    };
     long long group = gate ? r0 / a.group : 0;
     long long group_end = gate ? (group + 1) * a.group : r1;
     bool first_of_group = true, first = true;
     uint32_t slot = 0;
     for (long long r = r0; r < r1; ++r, slot = slot + 1 == a.stages ? 0 : slot + 1) {
         ring.advance();
-        const T* gate_row = gate ? gate + group * a.cols : nullptr;
         f2 hh[kPairs], v[kPairs], w[kPairs], t[kPairs];
         // hh = h rstd(h), v = x'
         cl.template read<false>(ring.read(slot, 0, r), hh);
@@ -373,12 +454,12 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             f2 ss = 0;
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(hh[k], hh[k], ss);
-            rh = rsqrtf(fmaf(block_sum(hsum(ss), 0.f).x, inv_n, a.eps));
+            rh = rsqrtf(fmaf(block_sum(hsum(ss)), inv_n, a.eps));
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) hh[k] = mul_f32x2(hh[k], dup(rh));
         }
-        cl.weights(wpost, w);
-        cl.weights(gate_row, t);
+        vector(keep_post, wpost, w);
+        vector(keep_gate, gate ? gate + group * a.cols : nullptr, t);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(mul_f32x2(hh[k], w[k]), mul_f32x2(t[k], dup(a.beta)));
         cl.template read<false>(ring.read(slot, 1, r), t);
@@ -387,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         // v = D
         if (wpre) {
             cl.template read<false>(ring.read(slot, 3, r), t);
-            cl.weights(wpre, w);
+            vector(keep_pre, wpre, w);
             f2 ss = 0, dot = 0;
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
@@ -418,24 +499,24 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         for (int k = 0; k < kPairs; ++k) t[k] = mul_f32x2(v[k], dup(a.alpha));
         cl.write(static_cast<T*>(a.dx) + r * a.cols, t);
         // dn = beta gate D and its sums
-        cl.weights(wpost, w);
+        vector(keep_post, wpost, w);
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], dup(a.beta));
         if (gate) {
             if constexpr (!REG) {
-                if (!first_of_group) cl.read_f32(my_gate + a.cols, s_gate);
+                if (!first_of_group) cl.read_f32(my_gate + a.part, s_gate);
                 else {
 #pragma unroll
                     for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
                 }
             }
-            cl.weights(gate_row, t);
+            vector(keep_gate, gate ? gate + group * a.cols : nullptr, t);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
                 s_gate[k] = fma_f32x2(v[k], mul_f32x2(hh[k], w[k]), s_gate[k]);
                 v[k] = mul_f32x2(v[k], t[k]);
             }
-            if constexpr (!REG) cl.write_f32(my_gate + a.cols, s_gate);
+            if constexpr (!REG) cl.write_f32(my_gate + a.part, s_gate);
         }
         if (wpost) {
             if constexpr (!REG) if (!first) cl.read_f32(my_post, s_post);
@@ -447,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
                 dot = fma_f32x2(v[k], hh[k], dot);
             }
             if constexpr (!REG) cl.write_f32(my_post, s_post);
-            const f2 mean = dup(-block_sum(hsum(dot), 0.f).x * inv_n);
+            const f2 mean = dup(-block_sum(hsum(dot)) * inv_n);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(fma_f32x2(hh[k], mean, v[k]), dup(rh));
         }
@@ -457,12 +538,13 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         if (gate && (r + 1 == group_end || r + 1 == r1)) {
             const long long begin = group * a.group;
             if (begin >= r0 && group_end <= r1) cl.write(static_cast<T*>(a.dgate) + group * a.cols, s_gate);
-            else cl.write_f32(my_gate + (begin < r0 ? 0 : a.cols), s_gate);
+            else cl.write_f32(my_gate + (begin < r0 ? 0 : a.part), s_gate);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
             first_of_group = true;
             ++group;
             group_end += a.group;
+            if constexpr (REG) if (r + 1 < r1) cl.keep(keep_gate, gate + group * a.cols);
         }
     }
     pdl_trigger();
@@ -473,55 +555,65 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
     cp_wait(0);
 }
 
-// Adds the CTAs' partial sums.  Item 0 is w_post, 1 is w_pre, 1 + c (0 < c < ctas)
-// the gate group that the border between CTAs c - 1 and c is the first to cut, if
-// there is one.  A block takes 32 columns; its 8 warps add every 8th CTA's row and
-// join them in order.
+// Adds the CTAs' partial sums.  Item 0 is w_post, 1 is w_pre, the others are gate
+// groups: 2 + g is group g (by_border == 0), or 1 + c the group that the border
+// between CTAs c - 1 and c is the first to cut, if there is one, so that there are at
+// most as many items as groups and as borders.  A block takes 128 columns, four per
+// lane; its SEGS warps add every SEGS-th CTA's row and are joined in order.
 struct SumArgs {
     const float *part_post, *part_pre, *part_gate;
     void *dw_post, *dw_pre, *dgate;
     long long per_cta, group;
-    uint32_t cols;
-    int ctas;
+    uint32_t cols, part;
+    int ctas, items, by_border;
 };
 
-template <typename T> __global__ void __launch_bounds__(256) norm_residual_sum_kernel(const SumArgs a) {
-    __shared__ float part[8][33];
-    const int cx = threadIdx.x & 31, seg = threadIdx.x >> 5;
-    const uint32_t col = blockIdx.x * 32 + cx;
+template <typename T, int SEGS> __global__ void __launch_bounds__(32 * SEGS) norm_residual_sum_kernel(const SumArgs a) {
+    __shared__ float4 part[SEGS][32];
+    const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
+    const uint32_t col = blockIdx.x * 128 + lane * 4;
     pdl_wait();
-    const int items = a.dgate ? a.ctas + 1 : 2;
-    for (int item = blockIdx.y; item < items; item += gridDim.y) {
+    for (int item = blockIdx.y; item < a.items; item += gridDim.y) {
         const float* src;
         T* dst;
-        long long c0 = 0, c1 = a.ctas, stride = a.cols, begin = 0;
+        int c0 = 0, c1 = a.ctas;
+        long long stride = a.part;
         if (item < 2) {
             src = item == 0 ? a.part_post : a.part_pre;
             dst = static_cast<T*>(item == 0 ? a.dw_post : a.dw_pre);
             if (!dst) continue;
         } else {
-            const long long border = static_cast<long long>(item - 1) * a.per_cta, g = border / a.group;
-            begin = g * a.group;
-            if (begin == border || begin < border - a.per_cta) continue;  // not cut here, or cut before
-            c0 = item - 2;
-            c1 = (begin + a.group - 1) / a.per_cta + 1;
+            const long long border = static_cast<long long>(item - 1) * a.per_cta;
+            const long long g = a.by_border ? border / a.group : item - 2, begin = g * a.group;
+            c0 = static_cast<int>(begin / a.per_cta);
+            c1 = static_cast<int>((begin + a.group - 1) / a.per_cta) + 1;
+            if (c1 - c0 == 1 || (a.by_border && c0 != item - 2)) continue;  // finished by its CTA, or not cut here first
             src = a.part_gate;
             dst = static_cast<T*>(a.dgate) + g * a.cols;
-            stride = 2 * static_cast<long long>(a.cols);
+            stride *= 2;
         }
-        float s = 0.f;
-        if (col < a.cols)
-            for (long long c = c0 + seg; c < c1; c += 8) {
-                // a CTA keeps the group that it begins inside of in its first slot, one that begins in it in its second
-                const uint32_t second = item >= 2 && c * a.per_cta <= begin ? a.cols : 0;
-                s += src[c * stride + second + col];
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (col < a.cols) {
+            const float* p = src + c0 * stride + col;
+            // a group's first CTA keeps it in its second slot (it begins there), the later ones in their first
+            const long long first = item >= 2 ? a.part : 0;
+#pragma unroll 8
+            for (int c = seg; c < c1 - c0; c += SEGS) {
+                const float4 v = *reinterpret_cast<const float4*>(p + c * stride + (c == 0 ? first : 0));
+                s.x += v.x;
+                s.y += v.y;
+                s.z += v.z;
+                s.w += v.w;
             }
-        part[seg][cx] = s;
+        }
+        part[seg][lane] = s;
         __syncthreads();
-        if (seg == 0 && col < a.cols) {
-#pragma unroll
-            for (int w = 1; w < 8; ++w) s += part[w][cx];
-            dst[col] = Conv<T>::down(s);
+        if (threadIdx.x < 128 && blockIdx.x * 128 + threadIdx.x < a.cols) {
+            const float* column = reinterpret_cast<const float*>(part) + threadIdx.x;
+            float t = 0.f;
+#pragma unroll 8
+            for (int w = 0; w < SEGS; ++w) t += column[w * 128];
+            dst[blockIdx.x * 128 + threadIdx.x] = Conv<T>::down(t);
         }
         __syncthreads();
     }
@@ -531,19 +623,20 @@ template <typename T> __global__ void __launch_bounds__(256) norm_residual_sum_k
 
 constexpr int kRingBytes = 200 * 1024;  // shared memory of one SM given to rings
 
-// Ring of a CTA when `per_sm` of them share an SM: up to 3 rows.
-void plan_ring(NormArgs& a, size_t elem, int tensors, int per_sm, bool vec) {
-    a.pitch = static_cast<uint32_t>((a.cols * elem + 15) / 16 * 16 + (vec ? 0 : 16));
-    const uint32_t slot = a.pitch * static_cast<uint32_t>(tensors);
-    const uint32_t fit = static_cast<uint32_t>(kRingBytes / per_sm) / slot;
-    a.stages = fit < 1 ? 1 : fit > 3 ? 3 : fit;
+// Ring of a CTA when `per_sm` of them share an SM: up to 3 rows of `tensors`
+// tensors beside `vectors` vectors.  Returns its bytes.
+int plan_ring(NormArgs& a, uint32_t pitch, int tensors, int vectors, int per_sm) {
+    a.pitch = pitch;
+    const int bytes = kRingBytes / per_sm - static_cast<int>(pitch) * vectors;
+    const int fit = bytes / static_cast<int>(pitch * static_cast<uint32_t>(tensors));
+    a.stages = fit < 1 ? 1 : fit > 3 ? 3 : static_cast<uint32_t>(fit);
+    return static_cast<int>(pitch) * (tensors * static_cast<int>(a.stages) + vectors);
 }
 
 template <typename T, bool VEC, int THREADS> int launch_fwd(NormArgs a, cudaStream_t st) {
     constexpr int per_sm = THREADS == 32 ? 24 : 1024 / THREADS;
-    plan_ring(a, sizeof(T), 2, per_sm, VEC);
+    const int smem = plan_ring(a, Cols<T, VEC, THREADS>::pitch(a.cols), 2, 0, per_sm);
     auto norm_kern = norm_residual_kernel<T, VEC, THREADS>;
-    const int smem = static_cast<int>(a.pitch * 2 * a.stages);
     static SmemLimit limit;
     if (int rc = limit.ensure(norm_kern, smem, "norm_gate_residual")) return rc;
     const long long cap = static_cast<long long>(sm_count()) * per_sm;
@@ -566,29 +659,33 @@ struct NormGrads {
 
 template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const NormGrads& g, cudaStream_t st) {
     constexpr int per_sm = THREADS == 32 ? 16 : THREADS <= 512 ? 512 / THREADS : 1;
-    plan_ring(a, sizeof(T), 4, per_sm, VEC);
+    const int smem = plan_ring(a, Cols<T, VEC, THREADS>::pitch(a.cols), 4, THREADS < 1024 ? 3 : 0, per_sm);
     auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS, (THREADS < 1024)>;
-    const int smem = static_cast<int>(a.pitch * 4 * a.stages);
     static SmemLimit limit;
     if (int rc = limit.ensure(norm_grad_kern, smem, "norm_gate_residual_backward")) return rc;
     const long long cap = static_cast<long long>(sm_count()) * per_sm;
     a.per_cta = (a.rows + cap - 1) / cap;
     const long long ctas = (a.rows + a.per_cta - 1) / a.per_cta;
-    const size_t bytes = static_cast<size_t>(a.cols) * static_cast<size_t>(ctas) * 4 * sizeof(float);
+    a.part = (a.cols + 3) / 4 * 4;
+    const size_t one = static_cast<size_t>(a.part) * static_cast<size_t>(ctas), bytes = one * 4 * sizeof(float);
     void* mem = nullptr;
     cudaError_t e = pool_malloc(&mem, bytes, st);
     if (e != cudaSuccess) return api_fail(e, "norm_gate_residual_backward: scratch of %zu bytes: %s", bytes, cudaGetErrorString(e));
     a.part_post = static_cast<float*>(mem);
-    a.part_pre = a.part_post + static_cast<size_t>(ctas) * a.cols;
-    a.part_gate = a.part_pre + static_cast<size_t>(ctas) * a.cols;
+    a.part_pre = a.part_post + one;
+    a.part_gate = a.part_pre + one;
     launch_pdl(norm_grad_kern, static_cast<unsigned>(ctas), THREADS, static_cast<size_t>(smem), st, a);
     int rc = launch_status("norm_gate_residual_backward");
     if (rc == 0) {
-        const SumArgs s{a.part_post, a.part_pre, a.part_gate, g.dw_post, g.dw_pre, g.dgate, a.per_cta, a.group, a.cols,
-                        static_cast<int>(ctas)};
-        const long long items = g.dgate ? ctas + 1 : 2;
-        const dim3 grid((a.cols + 31) / 32, static_cast<unsigned>(items < 64 ? items : 64));
-        launch_pdl(norm_residual_sum_kernel<T>, grid, 256, 0, st, s);
+        const long long groups = g.dgate ? a.rows / a.group : 0, borders = g.dgate ? ctas - 1 : 0;
+        const bool by_border = borders < groups;
+        const int items = 2 + static_cast<int>(by_border ? borders : groups);
+        const SumArgs s{a.part_post, a.part_pre, a.part_gate, g.dw_post, g.dw_pre, g.dgate, a.per_cta, a.group, a.cols, a.part,
+                        static_cast<int>(ctas), items, by_border ? 1 : 0};
+        const dim3 grid((a.cols + 127) / 128, static_cast<unsigned>(items < 256 ? items : 256));
+        // a warp adds a few dozen rows at most: 586 partial rows took 37 us with 8 warps, 147 take 5 us
+        if (ctas > 256) launch_pdl(norm_residual_sum_kernel<T, 32>, grid, 1024, 0, st, s);
+        else launch_pdl(norm_residual_sum_kernel<T, 8>, grid, 256, 0, st, s);
         rc = launch_status("norm_gate_residual_backward (sums)");
     }
     const cudaError_t e2 = cudaFreeAsync(mem, st);
