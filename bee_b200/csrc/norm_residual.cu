@@ -91,7 +91,7 @@ __device__ __forceinline__ void cp_wait(int pending) {
 // otherwise columns tid, tid + THREADS, ....  Columns past the row read as 0
 // and are not written, so they add nothing to any sum.
 template <typename T, bool VEC, int THREADS> struct Cols {
-    static constexpr int E = 16 / sizeof(T);
+    [[maybe_unused]] static constexpr int E = 16 / sizeof(T);
     uint32_t cols;
     __device__ __forceinline__ explicit Cols(uint32_t n) : cols(n) {}
     __device__ __forceinline__ static uint32_t vec(int j) { return j * THREADS + threadIdx.x; }
@@ -227,9 +227,15 @@ template <typename T, bool VEC, int THREADS> struct Cols {
 // Sums over the block with one barrier: consecutive calls use alternating halves
 // of `red`, so a call's writes never meet the previous call's reads.
 template <int THREADS> struct BlockSum {
-    static constexpr int WARPS = THREADS / 32;
-    f2 (*red)[WARPS];  // a warp's two sums, or one
+    static constexpr int WARPS = (THREADS / 32 + 3) / 4 * 4;  // those past the block's add 0
+    f2 (*red)[WARPS];  // rows 0 and 1: a warp's two sums; rows 2 and 3, as floats: its only one
     int parity = 0;
+    __device__ __forceinline__ explicit BlockSum(f2 (*r)[WARPS]) : red(r) {
+        if constexpr (THREADS / 32 < WARPS) {
+            for (int i = threadIdx.x; i < 4 * WARPS; i += THREADS) r[i / WARPS][i % WARPS] = 0;
+            __syncthreads();
+        }
+    }
     // of a and b, at once
     __device__ __forceinline__ float2 operator()(float a, float b) {
         a = warp_sum(a);
@@ -251,7 +257,7 @@ template <int THREADS> struct BlockSum {
     __device__ __forceinline__ float operator()(float a) {
         a = warp_sum(a);
         if constexpr (THREADS == 32) return a;
-        float* one = reinterpret_cast<float*>(red[parity]);
+        float* one = reinterpret_cast<float*>(red[2 + parity]);
         if ((threadIdx.x & 31) == 0) one[threadIdx.x >> 5] = a;
         __syncthreads();
         f2 r = 0;
@@ -351,8 +357,8 @@ struct NormArgs {
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ __align__(16) f2 red[2][THREADS / 32];
-    BlockSum<THREADS> block_sum{red};
+    __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
+    BlockSum<THREADS> block_sum(red);
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
     const long long r1 = r0 + a.per_cta < a.rows ? r0 + a.per_cta : a.rows;
@@ -403,13 +409,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
 
 // ---------------------------------------------------------------- backward
 
+// Whether the backward keeps w_post, w_pre and the gate in shared memory: 16-bit
+// ones do (L1 misses them beside the rings: 8192 columns 135 -> 105 us), fp32 ones and
+// the widest rows would take the ring's second stage (1111 columns in fp32: 37 us with, XX without).
+template <typename T> constexpr bool keep_vectors(int threads) { return sizeof(T) == 2 && threads < 1024; }
+
 // REG: the column sums stay in registers; otherwise (rows too wide for that) in
 // the CTA's own rows of the partial sums, read and written once per row.
 template <typename T, bool VEC, int THREADS, bool REG>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
+    constexpr bool KEEP = keep_vectors<T>(THREADS);
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ __align__(16) f2 red[2][THREADS / 32];
-    BlockSum<THREADS> block_sum{red};
+    __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
+    BlockSum<THREADS> block_sum(red);
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
     const long long r1 = r0 + a.per_cta < a.rows ? r0 + a.per_cta : a.rows;
@@ -424,20 +436,20 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
     f2 s_post[kPairs], s_pre[kPairs], s_gate[kPairs];
 #pragma unroll
     for (int k = 0; k < kPairs; ++k) s_post[k] = s_pre[k] = s_gate[k] = 0;
-    // the three vectors follow the ring, each thread's own columns (REG)
+    // the three vectors follow the ring, each thread's own columns (KEEP)
     T* keep_post = reinterpret_cast<T*>(ring_smem + a.pitch * 4 * a.stages);
     T* keep_pre = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 1));
     T* keep_gate = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 2));
     pdl_wait();
     ring.start(cl);
-    if constexpr (REG) {
+    if constexpr (KEEP) {
         cl.keep(keep_post, wpost);
         cl.keep(keep_pre, wpre);
         cl.keep(keep_gate, gate ? gate + r0 / a.group * a.cols : nullptr);
     }
-    // a vector's columns, from there or (rows too wide for that) from global memory
+    // a vector's columns, from there or from global memory
     auto vector = [&](const T* kept, const T* global, f2 (&out)[kPairs]) {
-        if constexpr (REG) cl.template read<false>(kept, out);
+        if constexpr (KEEP) cl.template read<false>(kept, out);
         else cl.weights(global, out);
     };
     long long group = gate ? r0 / a.group : 0;
@@ -544,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             first_of_group = true;
             ++group;
             group_end += a.group;
-            if constexpr (REG) if (r + 1 < r1) cl.keep(keep_gate, gate + group * a.cols);
+            if constexpr (KEEP) if (r + 1 < r1) cl.keep(keep_gate, gate + group * a.cols);
         }
     }
     pdl_trigger();
@@ -647,6 +659,8 @@ template <typename T, bool VEC, int THREADS> int launch_fwd(NormArgs a, cudaStre
 
 template <typename T, bool VEC> int forward(const NormArgs& a, cudaStream_t st) {
     if (a.cols <= 32 * kEpt) return launch_fwd<T, VEC, 32>(a, st);
+    if (a.cols <= 64 * kEpt) return launch_fwd<T, VEC, 64>(a, st);
+    if (a.cols <= 96 * kEpt) return launch_fwd<T, VEC, 96>(a, st);
     if (a.cols <= 128 * kEpt) return launch_fwd<T, VEC, 128>(a, st);
     if (a.cols <= 256 * kEpt) return launch_fwd<T, VEC, 256>(a, st);
     if (a.cols <= 512 * kEpt) return launch_fwd<T, VEC, 512>(a, st);
@@ -659,7 +673,7 @@ struct NormGrads {
 
 template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const NormGrads& g, cudaStream_t st) {
     constexpr int per_sm = THREADS == 32 ? 16 : THREADS <= 512 ? 512 / THREADS : 1;
-    const int smem = plan_ring(a, Cols<T, VEC, THREADS>::pitch(a.cols), 4, THREADS < 1024 ? 3 : 0, per_sm);
+    const int smem = plan_ring(a, Cols<T, VEC, THREADS>::pitch(a.cols), 4, keep_vectors<T>(THREADS) ? 3 : 0, per_sm);
     auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS, (THREADS < 1024)>;
     static SmemLimit limit;
     if (int rc = limit.ensure(norm_grad_kern, smem, "norm_gate_residual_backward")) return rc;
@@ -695,6 +709,8 @@ template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const No
 
 template <typename T, bool VEC> int backward(const NormArgs& a, const NormGrads& g, cudaStream_t st) {
     if (a.cols <= 32 * kEpt) return launch_bwd<T, VEC, 32>(a, g, st);
+    if (a.cols <= 64 * kEpt) return launch_bwd<T, VEC, 64>(a, g, st);
+    if (a.cols <= 96 * kEpt) return launch_bwd<T, VEC, 96>(a, g, st);
     if (a.cols <= 128 * kEpt) return launch_bwd<T, VEC, 128>(a, g, st);
     if (a.cols <= 256 * kEpt) return launch_bwd<T, VEC, 256>(a, g, st);
     if (a.cols <= 512 * kEpt) return launch_bwd<T, VEC, 512>(a, g, st);
