@@ -8,9 +8,9 @@
 // Wg, its peer the same columns of Wu, and the accumulator's halves are g and u
 // of the same outputs, so that the epilogue forms act(g) u from its own lanes.
 //
-// Forward, up to 128 rows (serving): bound by reading the weights once.  The
+// Forward, up to 64 rows (serving): bound by reading the weights once.  The
 // weights are the M operand (128 of their columns per CTA, for g and for u) and
-// the rows of x the N operand, padded only to 16, 32, 64 or 128.  Where the
+// the rows of x the N operand, padded only to 16, 32 or 64.  Where the
 // columns give too few CTAs, a cluster cuts K and joins its partial sums, in
 // rank order, through distributed shared memory.
 //
@@ -702,7 +702,8 @@ int launch_pair(const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, Pair
     return launch_status(what);
 }
 
-constexpr int kFewRows = 128;
+// 128 rows: 66.8 us there, 64 as one tile of the pair kernel (4096 -> 14336)
+constexpr int kFewRows = 64;
 
 template <int NT, bool W_MN> int launch_rows(const Mat& x, const Mat& g, const Mat& u, RowsParams p, const char* what, cudaStream_t st) {
     constexpr int STAGE = 2 * 128 * 64 * 2 + NT * 64 * 2;
@@ -711,14 +712,25 @@ template <int NT, bool W_MN> int launch_rows(const Mat& x, const Mat& g, const M
     if (int rc = map_of(&tx, x, NT, f16)) return rc;
     if (int rc = map_of(&tg, g, W_MN ? 64 : 128, f16)) return rc;
     if (int rc = map_of(&tu, u, W_MN ? 64 : 128, f16)) return rc;
-    const int tiles = (p.N + 127) / 128, sms = sm_count();
-    p.cluster = 1;
-    while (p.cluster < 8 && tiles * p.cluster * 10 < sms * 7 && p.num_kb >= 8 * p.cluster) p.cluster *= 2;
-    // deep rings for one CTA per SM, half as deep for two
+    // Deep rings for one CTA per SM, half as deep for two (which also hold the partial sums).
     constexpr int ONE = (220 * 1024) / STAGE < 6 ? (220 * 1024) / STAGE : 6;
     constexpr int TWO = (109 * 1024) / STAGE;
-    constexpr bool two_fit = TWO * STAGE >= 2 * NT * 128 * 4;  // the partial sums share the ring's memory
-    p.stages = two_fit && tiles * p.cluster > sms ? TWO : ONE;
+    constexpr int resident = TWO * STAGE >= 2 * NT * 128 * 4 ? 2 : 1;
+    // One SM draws about 50 GB/s whatever its ring, so the time is that of the SM with the most work: the cut of
+    // K is the one whose busiest SM has the least, the finer one if equal (14336 columns, one row: 41.9 us uncut with
+    // one CTA per SM, 39.2 cut in two; 11008 columns, 48 rows: 44.5 us uncut, 43.7 in two, 37.3 in three).
+    const int tiles = (p.N + 127) / 128, sms = sm_count();
+    p.cluster = 1;
+    double least = 0;
+    for (int cut = 1; cut <= 8 && (cut == 1 || (tiles * cut <= resident * sms && p.num_kb >= 4 * cut)); ++cut) {
+        const int ctas = tiles * cut;
+        const double busiest = static_cast<double>((ctas + sms - 1) / sms) / ctas;
+        if (cut == 1 || busiest <= least) {
+            least = busiest;
+            p.cluster = cut;
+        }
+    }
+    p.stages = tiles * p.cluster > sms && resident == 2 ? TWO : ONE;
     const int smem = p.stages * STAGE + 1024;
     auto gated_rows = gated_rows_kernel<NT, W_MN>;
     static SmemLimit limit;
@@ -735,8 +747,7 @@ template <int NT, bool W_MN> int launch_rows(const Mat& x, const Mat& g, const M
 template <bool W_MN> int forward_rows(const Mat& x, const Mat& g, const Mat& u, const RowsParams& p, const char* what, cudaStream_t st) {
     if (p.M <= 16) return launch_rows<16, W_MN>(x, g, u, p, what, st);
     if (p.M <= 32) return launch_rows<32, W_MN>(x, g, u, p, what, st);
-    if (p.M <= 64) return launch_rows<64, W_MN>(x, g, u, p, what, st);
-    return launch_rows<128, W_MN>(x, g, u, p, what, st);
+    return launch_rows<64, W_MN>(x, g, u, p, what, st);
 }
 
 int check(const char* what, int dt, int act, size_t M, size_t D, size_t F, size_t ldx, size_t ldw, bool trans) {

@@ -348,7 +348,7 @@ BEE_B200_API int bee_b200_bmm_strided(int dt_in, int dt_out, const void* A, int6
  * they may be two slices of one fused matrix.  g and u (both or neither, [M, F]
  * contiguous): x Wg and x Wu, kept for the backward.  act: 0 silu, 1 gelu (erf),
  * 2 gelu (tanh).  dt in {BF16, F16}; fp32 accumulation on the tensor cores, one
- * rounding per output (out from the unrounded products).  Up to 128 rows run a
+ * rounding per output (out from the unrounded products).  Up to 64 rows run a
  * kernel that is bound by reading the weights once.  Operands whose rows are not 16-byte
  * aligned are copied to padded scratch first (2 bytes an element of them, from
  * the stream-ordered pool). */
