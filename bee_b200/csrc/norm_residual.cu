@@ -16,11 +16,11 @@
 // Both are bound by HBM (forward: 2 reads and 2 writes of the tensor, backward:
 // 4 and 2).  A CTA owns whole rows, so every tensor crosses HBM once: upcoming
 // rows are copied into a shared-memory ring with cp.async while the current one
-// is reduced (1 or 2 block reductions forward, 3 backward).  All arithmetic is
+// is reduced (1 or 2 block reductions a row).  All arithmetic is
 // fp32, in packed pairs; results are rounded once, when stored.
 //
-// A thread owns the same kEpt = 16 columns of every row, so the backward's three
-// column sums stay in registers over the CTA's contiguous range of rows; each CTA
+// A thread owns the same kEpt = 16 columns of every row, so the backward's column
+// sums stay in registers over the CTA's contiguous range of rows; each CTA
 // writes one row of partial sums and a second kernel adds them in a fixed order
 // (results do not depend on timing).  A group of rows that lies inside one
 // CTA's range is finished there; one that is cut leaves a partial per CTA.
@@ -409,16 +409,18 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
 
 // ---------------------------------------------------------------- backward
 
-// Whether the backward keeps w_post, w_pre and the gate in shared memory: 16-bit
-// ones do (L1 misses them beside the rings: 8192 columns 135 -> 105 us), fp32 ones and
-// the widest rows would take the ring's second stage (1111 columns in fp32: 37 us with, XX without).
-template <typename T> constexpr bool keep_vectors(int threads) { return sizeof(T) == 2 && threads < 1024; }
+// Whether the backward keeps beta gate w_post (in fp32) and w_pre in shared memory:
+// L1 misses the vectors beside the rings, and each use would unpack and multiply them
+// again (8192 x 4096 fp32: 144 us without, 135 with).  The widest rows need the room for the ring.
+constexpr bool keep_vectors(int threads) { return threads < 1024; }
 
+// w_post and the gate share a column sum: with P = sum over a group's rows of D hh,
+// dgate = beta w_post P, and dw_post is the sum over the groups of beta gate P.
 // REG: the column sums stay in registers; otherwise (rows too wide for that) in
 // the CTA's own rows of the partial sums, read and written once per row.
 template <typename T, bool VEC, int THREADS, bool REG>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
-    constexpr bool KEEP = keep_vectors<T>(THREADS);
+    constexpr bool KEEP = keep_vectors(THREADS);
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
     BlockSum<THREADS> block_sum(red);
@@ -433,59 +435,80 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
     float* my_post = a.part_post + static_cast<long long>(blockIdx.x) * a.part;
     float* my_pre = a.part_pre + static_cast<long long>(blockIdx.x) * a.part;
     float* my_gate = a.part_gate + static_cast<long long>(blockIdx.x) * 2 * a.part;
-    f2 s_post[kPairs], s_pre[kPairs], s_gate[kPairs];
+    f2 s_col[kPairs], s_pre[kPairs];  // sums of D hh (this group's rows) and of dy xh
 #pragma unroll
-    for (int k = 0; k < kPairs; ++k) s_post[k] = s_pre[k] = s_gate[k] = 0;
-    // the three vectors follow the ring, each thread's own columns (KEEP)
-    T* keep_post = reinterpret_cast<T*>(ring_smem + a.pitch * 4 * a.stages);
-    T* keep_pre = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 1));
-    T* keep_gate = reinterpret_cast<T*>(ring_smem + a.pitch * (4 * a.stages + 2));
+    for (int k = 0; k < kPairs; ++k) s_col[k] = s_pre[k] = 0;
+    // KEEP: after the ring, w_pre and then beta gate w_post, of which a thread reads only what it wrote
+    T* kept_pre = reinterpret_cast<T*>(ring_smem + a.pitch * 4 * a.stages);
+    ulonglong2* kept_factor = reinterpret_cast<ulonglong2*>(ring_smem + a.pitch * (4 * a.stages + 1)) + threadIdx.x;
+    long long group = gate ? r0 / a.group : 0;
+    long long group_end = gate ? (group + 1) * a.group : r1;
+    // beta gate w_post of the current group, from global memory
+    auto load_factor = [&](f2 (&f)[kPairs]) {
+        f2 t[kPairs];
+        cl.weights(wpost, f);
+        cl.weights(gate ? gate + group * a.cols : nullptr, t);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) f[k] = mul_f32x2(f[k], mul_f32x2(t[k], dup(a.beta)));
+    };
+    auto keep_factor = [&] {
+        f2 f[kPairs];
+        load_factor(f);
+#pragma unroll
+        for (int k = 0; k < kPairs; k += 2) kept_factor[k / 2 * THREADS] = make_ulonglong2(f[k], f[k + 1]);
+    };
+    auto factor = [&](f2 (&f)[kPairs]) {
+        if constexpr (KEEP) {
+#pragma unroll
+            for (int k = 0; k < kPairs; k += 2) {
+                const ulonglong2 q = kept_factor[k / 2 * THREADS];
+                f[k] = q.x;
+                f[k + 1] = q.y;
+            }
+        } else {
+            load_factor(f);
+        }
+    };
+    auto squares = [&](const T* row) {
+        f2 v[kPairs], ss = 0;
+        cl.template read<false>(row, v);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(v[k], v[k], ss);
+        return hsum(ss);
+    };
     pdl_wait();
     ring.start(cl);
     if constexpr (KEEP) {
-        cl.keep(keep_post, wpost);
-        cl.keep(keep_pre, wpre);
-        cl.keep(keep_gate, gate ? gate + r0 / a.group * a.cols : nullptr);
+        cl.keep(kept_pre, wpre);
+        keep_factor();
     }
-    // a vector's columns, from there or from global memory
-    auto vector = [&](const T* kept, const T* global, f2 (&out)[kPairs]) {
-        if constexpr (KEEP) cl.template read<false>(kept, out);
-        else cl.weights(global, out);
-    };
-    long long group = gate ? r0 / a.group : 0;
-    long long group_end = gate ? (group + 1) * a.group : r1;
-    bool first_of_group = true, first = true;
+    bool first = true, first_of_group = true, first_group = true;
     uint32_t slot = 0;
-    for (long long r = r0; r < r1; ++r, slot = slot + 1 == a.stages ? 0 : slot + 1) {
-        ring.advance();
+    float rh = 1.f;  // of the current row; found with the sums of the row before
+    ring.advance();
+    if (wpost) rh = rsqrtf(fmaf(block_sum(squares(ring.read(0, 0, r0))), inv_n, a.eps));
+    for (long long r = r0; r < r1; ++r) {
         f2 hh[kPairs], v[kPairs], w[kPairs], t[kPairs];
         // hh = h rstd(h), v = x'
         cl.template read<false>(ring.read(slot, 0, r), hh);
-        float rh = 1.f;
-        if (wpost) {
-            f2 ss = 0;
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) ss = fma_f32x2(hh[k], hh[k], ss);
-            rh = rsqrtf(fmaf(block_sum(hsum(ss)), inv_n, a.eps));
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) hh[k] = mul_f32x2(hh[k], dup(rh));
-        }
-        vector(keep_post, wpost, w);
-        vector(keep_gate, gate ? gate + group * a.cols : nullptr, t);
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(mul_f32x2(hh[k], w[k]), mul_f32x2(t[k], dup(a.beta)));
+        factor(w);
         cl.template read<false>(ring.read(slot, 1, r), t);
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) v[k] = fma_f32x2(t[k], dup(a.alpha), v[k]);
+        for (int k = 0; k < kPairs; ++k) {
+            hh[k] = mul_f32x2(hh[k], dup(rh));
+            v[k] = fma_f32x2(hh[k], w[k], mul_f32x2(t[k], dup(a.alpha)));
+        }
         // v = D
         if (wpre) {
             cl.template read<false>(ring.read(slot, 3, r), t);
-            vector(keep_pre, wpre, w);
+            if constexpr (KEEP) cl.template read<false>(kept_pre, w);
+            else cl.weights(wpre, w);
             f2 ss = 0, dot = 0;
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
                 ss = fma_f32x2(v[k], v[k], ss);
-                dot = fma_f32x2(mul_f32x2(t[k], w[k]), v[k], dot);
+                w[k] = mul_f32x2(t[k], w[k]);
+                dot = fma_f32x2(w[k], v[k], dot);
             }
             const float2 sum = block_sum(hsum(ss), hsum(dot));
             const float rx = rsqrtf(fmaf(sum.x, inv_n, a.eps));
@@ -495,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             for (int k = 0; k < kPairs; ++k) {
                 const f2 xh = mul_f32x2(v[k], rx2);
                 s_pre[k] = fma_f32x2(t[k], xh, s_pre[k]);
-                v[k] = mul_f32x2(fma_f32x2(xh, mean, mul_f32x2(t[k], w[k])), rx2);
+                v[k] = mul_f32x2(fma_f32x2(xh, mean, w[k]), rx2);
             }
             if constexpr (!REG) cl.write_f32(my_pre, s_pre);
         } else {
@@ -510,58 +533,59 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) t[k] = mul_f32x2(v[k], dup(a.alpha));
         cl.write(static_cast<T*>(a.dx) + r * a.cols, t);
-        // dn = beta gate D and its sums
-        vector(keep_post, wpost, w);
+        // the group's column sum, and v = dn w_post with dn = beta gate D
+        if constexpr (!REG) if (!first_of_group) cl.read_f32(my_gate + a.part, s_col);
+        factor(w);
+        f2 dot = 0;
 #pragma unroll
-        for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(v[k], dup(a.beta));
-        if (gate) {
-            if constexpr (!REG) {
-                if (!first_of_group) cl.read_f32(my_gate + a.part, s_gate);
-                else {
-#pragma unroll
-                    for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
-                }
-            }
-            vector(keep_gate, gate ? gate + group * a.cols : nullptr, t);
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-                s_gate[k] = fma_f32x2(v[k], mul_f32x2(hh[k], w[k]), s_gate[k]);
-                v[k] = mul_f32x2(v[k], t[k]);
-            }
-            if constexpr (!REG) cl.write_f32(my_gate + a.part, s_gate);
+        for (int k = 0; k < kPairs; ++k) {
+            s_col[k] = fma_f32x2(v[k], hh[k], s_col[k]);
+            v[k] = mul_f32x2(v[k], w[k]);
+            dot = fma_f32x2(v[k], hh[k], dot);
         }
+        if constexpr (!REG) cl.write_f32(my_gate + a.part, s_col);
+        // on to the next row (this one's slot has been read), whose sum of squares joins this row's last sum
+        const bool more = r + 1 < r1;
+        slot = slot + 1 == a.stages ? 0 : slot + 1;
+        if (more) ring.advance();
         if (wpost) {
-            if constexpr (!REG) if (!first) cl.read_f32(my_post, s_post);
-            f2 dot = 0;
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) {
-                s_post[k] = fma_f32x2(v[k], hh[k], s_post[k]);
-                v[k] = mul_f32x2(v[k], w[k]);
-                dot = fma_f32x2(v[k], hh[k], dot);
-            }
-            if constexpr (!REG) cl.write_f32(my_post, s_post);
-            const f2 mean = dup(-block_sum(hsum(dot)) * inv_n);
+            const float2 sum = block_sum(hsum(dot), more ? squares(ring.read(slot, 0, r + 1)) : 0.f);
+            const f2 mean = dup(-sum.x * inv_n);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v[k] = mul_f32x2(fma_f32x2(hh[k], mean, v[k]), dup(rh));
+            rh = rsqrtf(fmaf(sum.y, inv_n, a.eps));
         }
         cl.write(static_cast<T*>(a.dh) + r * a.cols, v);
         first = first_of_group = false;
-        // the group ends here: finished if it began in this range, else a partial sum
-        if (gate && (r + 1 == group_end || r + 1 == r1)) {
-            const long long begin = group * a.group;
-            if (begin >= r0 && group_end <= r1) cl.write(static_cast<T*>(a.dgate) + group * a.cols, s_gate);
-            else cl.write_f32(my_gate + (begin < r0 ? 0 : a.part), s_gate);
+        if (r + 1 == group_end || !more) {
 #pragma unroll
-            for (int k = 0; k < kPairs; ++k) s_gate[k] = 0;
+            for (int k = 0; k < kPairs; ++k) s_col[k] = mul_f32x2(s_col[k], dup(a.beta));
+            if (wpost) {
+                cl.weights(gate ? gate + group * a.cols : nullptr, w);
+                if (!first_group) cl.read_f32(my_post, t);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) w[k] = fma_f32x2(w[k], s_col[k], first_group ? 0 : t[k]);
+                cl.write_f32(my_post, w);
+            }
+            if (gate) {  // the group is finished if it began in this range, else this is a partial sum
+                const long long begin = group * a.group;
+                cl.weights(wpost, w);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) w[k] = mul_f32x2(w[k], s_col[k]);
+                if (begin >= r0 && group_end <= r1) cl.write(static_cast<T*>(a.dgate) + group * a.cols, w);
+                else cl.write_f32(my_gate + (begin < r0 ? 0 : a.part), w);
+            }
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) s_col[k] = 0;
             first_of_group = true;
+            first_group = false;
             ++group;
             group_end += a.group;
-            if constexpr (KEEP) if (r + 1 < r1) cl.keep(keep_gate, gate + group * a.cols);
+            if constexpr (KEEP) if (more) keep_factor();
         }
     }
     pdl_trigger();
     if constexpr (REG) {
-        if (wpost) cl.write_f32(my_post, s_post);
         if (wpre) cl.write_f32(my_pre, s_pre);
     }
     cp_wait(0);
@@ -636,13 +660,12 @@ template <typename T, int SEGS> __global__ void __launch_bounds__(32 * SEGS) nor
 constexpr int kRingBytes = 200 * 1024;  // shared memory of one SM given to rings
 
 // Ring of a CTA when `per_sm` of them share an SM: up to 3 rows of `tensors`
-// tensors beside `vectors` vectors.  Returns its bytes.
-int plan_ring(NormArgs& a, uint32_t pitch, int tensors, int vectors, int per_sm) {
+// tensors beside `kept` bytes.  Returns the bytes of both.
+int plan_ring(NormArgs& a, uint32_t pitch, int tensors, int kept, int per_sm) {
     a.pitch = pitch;
-    const int bytes = kRingBytes / per_sm - static_cast<int>(pitch) * vectors;
-    const int fit = bytes / static_cast<int>(pitch * static_cast<uint32_t>(tensors));
+    const int slot = static_cast<int>(pitch) * tensors, fit = (kRingBytes / per_sm - kept) / slot;
     a.stages = fit < 1 ? 1 : fit > 3 ? 3 : static_cast<uint32_t>(fit);
-    return static_cast<int>(pitch) * (tensors * static_cast<int>(a.stages) + vectors);
+    return slot * static_cast<int>(a.stages) + kept;
 }
 
 template <typename T, bool VEC, int THREADS> int launch_fwd(NormArgs a, cudaStream_t st) {
@@ -673,7 +696,9 @@ struct NormGrads {
 
 template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const NormGrads& g, cudaStream_t st) {
     constexpr int per_sm = THREADS == 32 ? 16 : THREADS <= 512 ? 512 / THREADS : 1;
-    const int smem = plan_ring(a, Cols<T, VEC, THREADS>::pitch(a.cols), 4, keep_vectors<T>(THREADS) ? 3 : 0, per_sm);
+    const uint32_t pitch = Cols<T, VEC, THREADS>::pitch(a.cols);
+    const int kept = keep_vectors(THREADS) ? static_cast<int>(pitch) + THREADS * kEpt * 4 : 0;
+    const int smem = plan_ring(a, pitch, 4, kept, per_sm);
     auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS, (THREADS < 1024)>;
     static SmemLimit limit;
     if (int rc = limit.ensure(norm_grad_kern, smem, "norm_gate_residual_backward")) return rc;
