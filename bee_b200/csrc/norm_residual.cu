@@ -41,7 +41,7 @@ namespace {
 
 constexpr int kEpt = 16;         // columns per thread
 constexpr int kPairs = kEpt / 2;
-// 1024 threads' columns; in fp32, what the four rows of a backward slot leave in shared memory
+// 1024 threads' columns; in fp32 768 threads', since the four rows of a backward slot fill the shared memory
 constexpr size_t max_cols(int dt) { return dt == DT_F32 ? 12288 : 16384; }
 using f2 = uint64_t;             // two fp32 values
 
@@ -412,15 +412,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(
 // Whether the backward keeps beta gate w_post (in fp32) and w_pre in shared memory:
 // L1 misses the vectors beside the rings, and each use would unpack and multiply them
 // again (8192 x 4096 fp32: 144 us without, 135 with).  The widest rows need the room for the ring.
-constexpr bool keep_vectors(int threads) { return threads < 1024; }
+template <typename T> constexpr bool keep_vectors(int threads) { return threads < (sizeof(T) == 2 ? 1024 : 768); }
 
 // w_post and the gate share a column sum: with P = sum over a group's rows of D hh,
 // dgate = beta w_post P, and dw_post is the sum over the groups of beta gate P.
-// REG: the column sums stay in registers; otherwise (rows too wide for that) in
-// the CTA's own rows of the partial sums, read and written once per row.
-template <typename T, bool VEC, int THREADS, bool REG>
+// From 768 threads on the column sums leave too few registers and some spill
+// (4096 x 12288 bf16: 201 us with 768 threads, 295 with 1024, 549 with the sums in memory).
+template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
-    constexpr bool KEEP = keep_vectors(THREADS);
+    constexpr bool KEEP = keep_vectors<T>(THREADS);
     extern __shared__ __align__(16) uint8_t ring_smem[];
     __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
     BlockSum<THREADS> block_sum(red);
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         cl.keep(kept_pre, wpre);
         keep_factor();
     }
-    bool first = true, first_of_group = true, first_group = true;
+    bool first_group = true;
     uint32_t slot = 0;
     float rh = 1.f;  // of the current row; found with the sums of the row before
     ring.advance();
@@ -513,14 +513,12 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             const float2 sum = block_sum(hsum(ss), hsum(dot));
             const float rx = rsqrtf(fmaf(sum.x, inv_n, a.eps));
             const f2 rx2 = dup(rx), mean = dup(-rx * sum.y * inv_n);  // -mean(dy w_pre xh)
-            if constexpr (!REG) if (!first) cl.read_f32(my_pre, s_pre);
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) {
                 const f2 xh = mul_f32x2(v[k], rx2);
                 s_pre[k] = fma_f32x2(t[k], xh, s_pre[k]);
                 v[k] = mul_f32x2(fma_f32x2(xh, mean, w[k]), rx2);
             }
-            if constexpr (!REG) cl.write_f32(my_pre, s_pre);
         } else {
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) v[k] = 0;
@@ -534,7 +532,6 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         for (int k = 0; k < kPairs; ++k) t[k] = mul_f32x2(v[k], dup(a.alpha));
         cl.write(static_cast<T*>(a.dx) + r * a.cols, t);
         // the group's column sum, and v = dn w_post with dn = beta gate D
-        if constexpr (!REG) if (!first_of_group) cl.read_f32(my_gate + a.part, s_col);
         factor(w);
         f2 dot = 0;
 #pragma unroll
@@ -543,7 +540,6 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             v[k] = mul_f32x2(v[k], w[k]);
             dot = fma_f32x2(v[k], hh[k], dot);
         }
-        if constexpr (!REG) cl.write_f32(my_gate + a.part, s_col);
         // on to the next row (this one's slot has been read), whose sum of squares joins this row's last sum
         const bool more = r + 1 < r1;
         slot = slot + 1 == a.stages ? 0 : slot + 1;
@@ -556,7 +552,6 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             rh = rsqrtf(fmaf(sum.y, inv_n, a.eps));
         }
         cl.write(static_cast<T*>(a.dh) + r * a.cols, v);
-        first = first_of_group = false;
         if (r + 1 == group_end || !more) {
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) s_col[k] = mul_f32x2(s_col[k], dup(a.beta));
@@ -577,7 +572,6 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
             }
 #pragma unroll
             for (int k = 0; k < kPairs; ++k) s_col[k] = 0;
-            first_of_group = true;
             first_group = false;
             ++group;
             group_end += a.group;
@@ -585,9 +579,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
         }
     }
     pdl_trigger();
-    if constexpr (REG) {
-        if (wpre) cl.write_f32(my_pre, s_pre);
-    }
+    if (wpre) cl.write_f32(my_pre, s_pre);
     cp_wait(0);
 }
 
@@ -685,9 +677,14 @@ template <typename T, bool VEC> int forward(const NormArgs& a, cudaStream_t st) 
     if (a.cols <= 64 * kEpt) return launch_fwd<T, VEC, 64>(a, st);
     if (a.cols <= 96 * kEpt) return launch_fwd<T, VEC, 96>(a, st);
     if (a.cols <= 128 * kEpt) return launch_fwd<T, VEC, 128>(a, st);
+    if (a.cols <= 160 * kEpt) return launch_fwd<T, VEC, 160>(a, st);
     if (a.cols <= 256 * kEpt) return launch_fwd<T, VEC, 256>(a, st);
+    if (a.cols <= 320 * kEpt) return launch_fwd<T, VEC, 320>(a, st);
+    if (a.cols <= 384 * kEpt) return launch_fwd<T, VEC, 384>(a, st);
     if (a.cols <= 512 * kEpt) return launch_fwd<T, VEC, 512>(a, st);
-    return launch_fwd<T, VEC, 1024>(a, st);
+    if (sizeof(T) == 4 || a.cols <= 768 * kEpt) return launch_fwd<T, VEC, 768>(a, st);
+    if constexpr (sizeof(T) == 2) return launch_fwd<T, VEC, 1024>(a, st);
+    return fail(cudaErrorInvalidValue, "norm_gate_residual: %u columns", a.cols);  // refused before
 }
 
 struct NormGrads {
@@ -697,9 +694,9 @@ struct NormGrads {
 template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const NormGrads& g, cudaStream_t st) {
     constexpr int per_sm = THREADS == 32 ? 16 : THREADS <= 512 ? 512 / THREADS : 1;
     const uint32_t pitch = Cols<T, VEC, THREADS>::pitch(a.cols);
-    const int kept = keep_vectors(THREADS) ? static_cast<int>(pitch) + THREADS * kEpt * 4 : 0;
+    const int kept = keep_vectors<T>(THREADS) ? static_cast<int>(pitch) + THREADS * kEpt * 4 : 0;
     const int smem = plan_ring(a, pitch, 4, kept, per_sm);
-    auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS, (THREADS < 1024)>;
+    auto norm_grad_kern = norm_residual_grad_kernel<T, VEC, THREADS>;
     static SmemLimit limit;
     if (int rc = limit.ensure(norm_grad_kern, smem, "norm_gate_residual_backward")) return rc;
     const long long cap = static_cast<long long>(sm_count()) * per_sm;
@@ -737,9 +734,14 @@ template <typename T, bool VEC> int backward(const NormArgs& a, const NormGrads&
     if (a.cols <= 64 * kEpt) return launch_bwd<T, VEC, 64>(a, g, st);
     if (a.cols <= 96 * kEpt) return launch_bwd<T, VEC, 96>(a, g, st);
     if (a.cols <= 128 * kEpt) return launch_bwd<T, VEC, 128>(a, g, st);
+    if (a.cols <= 160 * kEpt) return launch_bwd<T, VEC, 160>(a, g, st);
     if (a.cols <= 256 * kEpt) return launch_bwd<T, VEC, 256>(a, g, st);
+    if (a.cols <= 320 * kEpt) return launch_bwd<T, VEC, 320>(a, g, st);
+    if (a.cols <= 384 * kEpt) return launch_bwd<T, VEC, 384>(a, g, st);
     if (a.cols <= 512 * kEpt) return launch_bwd<T, VEC, 512>(a, g, st);
-    return launch_bwd<T, VEC, 1024>(a, g, st);
+    if (sizeof(T) == 4 || a.cols <= 768 * kEpt) return launch_bwd<T, VEC, 768>(a, g, st);
+    if constexpr (sizeof(T) == 2) return launch_bwd<T, VEC, 1024>(a, g, st);
+    return fail(cudaErrorInvalidValue, "norm_gate_residual: %u columns", a.cols);  // refused before
 }
 
 int check(const char* what, int dt, size_t rows, size_t cols, size_t group, bool gate, float alpha, float beta, float eps) {

@@ -115,7 +115,7 @@ def check_all(torch, s, alpha=0.75, beta=1.25):
 
 # widths around the vector, the warp and each block size; rows below, at and above one per CTA
 SHAPES = [(1, 1), (2, 3), (3, 8), (1, 64), (40, 100), (7, 512), (500, 513), (3, 1000), (9, 1024), (600, 1100), (20, 1536), (1, 2048), (310, 2056), (11, 2049),
-          (150, 4096), (5, 4100), (450, 4104), (2, 8192), (151, 8200), (3, 8193), (5, 12288)]
+          (150, 4096), (5, 4100), (450, 4104), (2, 2560), (9, 5120), (160, 6000), (2, 8192), (151, 8200), (3, 8193), (5, 12288)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
