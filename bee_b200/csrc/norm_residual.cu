@@ -115,17 +115,20 @@ template <typename T, bool VEC, int THREADS> struct Cols {
             return make_uint4(Conv<T>::down2(v[0]), Conv<T>::down2(v[1]), Conv<T>::down2(v[2]), Conv<T>::down2(v[3]));
         }
     }
-    // bytes of a row in a ring slot
-    static constexpr bool kPadded = VEC && THREADS < 1024;  // slots as wide as the block's columns, zero past the row's end
+    // Slots as wide as the block's columns, zero past the row's end, so that they are read without bounds; the
+    // widest rows have exact ones.  Bytes of a row in a slot (its first 16-byte block may begin before the row):
+    static constexpr bool kPadded = THREADS < 1024;
     static __host__ __device__ constexpr uint32_t pitch(uint32_t cols) {
-        return kPadded ? THREADS * kEpt * sizeof(T) : (cols * static_cast<uint32_t>(sizeof(T)) + 15) / 16 * 16 + (VEC ? 0 : 16);
+        return (kPadded ? THREADS * kEpt * static_cast<uint32_t>(sizeof(T)) : (cols * static_cast<uint32_t>(sizeof(T)) + 15) / 16 * 16) + (VEC ? 0 : 16);
     }
-    // zeros where this thread's vectors of a slot lie past the row's end
+    // zeros in a slot: VEC, this thread's own vectors past the row's end; else this thread's share of all of it
     __device__ __forceinline__ void pad(uint8_t* slot) const {
-        if constexpr (kPadded) {
+        if constexpr (kPadded && VEC) {
 #pragma unroll
             for (int j = 0; j < kEpt / E; ++j)
                 if (vec(j) * E >= cols) reinterpret_cast<uint4*>(slot)[vec(j)] = make_uint4(0, 0, 0, 0);
+        } else if constexpr (kPadded) {
+            for (uint32_t i = threadIdx.x; i < pitch(cols) / 16; i += THREADS) reinterpret_cast<uint4*>(slot)[i] = make_uint4(0, 0, 0, 0);
         }
     }
     // this thread's columns of an optional vector into a slot (absent: ones), which only this thread reads
@@ -146,16 +149,19 @@ template <typename T, bool VEC, int THREADS> struct Cols {
             for (int k = 0; k < kPairs; ++k) {
                 float a, b;
                 unpack_f32x2(v[k], a, b);
-                if (col(2 * k) < cols) slot[col(2 * k)] = Conv<T>::down(a);
-                if (col(2 * k + 1) < cols) slot[col(2 * k + 1)] = Conv<T>::down(b);
+                if (kPadded || col(2 * k) < cols) slot[col(2 * k)] = Conv<T>::down(a);
+                if (kPadded || col(2 * k + 1) < cols) slot[col(2 * k + 1)] = Conv<T>::down(b);
             }
         }
     }
     // from a row (shared or global memory; LDG: read-only global vectors)
     template <bool LDG> __device__ __forceinline__ void read(const T* p, f2 (&v)[kPairs]) const {
-        if constexpr (kPadded && !LDG) {
+        if constexpr (kPadded && VEC && !LDG) {
 #pragma unroll
             for (int j = 0; j < kEpt / E; ++j) unpack(reinterpret_cast<const uint4*>(p)[vec(j)], v + j * (E / 2));
+        } else if constexpr (kPadded && !LDG) {
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) v[k] = pack_f32x2(Conv<T>::up(p[col(2 * k)]), Conv<T>::up(p[col(2 * k + 1)]));
         } else if constexpr (VEC) {
 #pragma unroll
             for (int j = 0; j < kEpt / E; ++j) {
@@ -302,16 +308,20 @@ template <typename T, bool VEC, int THREADS, int NT> struct Ring {
                         if (v * E < cols) cp_async16(dst + v * 16, reinterpret_cast<const uint4*>(g) + v, 16);
                     }
                 } else {
-                    // the 16-byte blocks that cover the row; the last is cut at the row's end, and one
-                    // that begins before the tensor is copied element by element
+                    // the 16-byte blocks that cover the row; the last is cut at the row's end (zeros follow), one
+                    // that begins before the tensor is copied element by element, and one of zeros comes after
+                    // them: the row before may have ended later in this slot, by less than a block
                     const uint32_t ld = lead(t, row), bytes = ld + cols * static_cast<uint32_t>(sizeof(T));
                     const uint8_t* a = reinterpret_cast<const uint8_t*>(g) - ld;
-                    for (uint32_t o = threadIdx.x * 16; o < bytes; o += THREADS * 16) {
+                    const uint32_t filled = (bytes + 15) / 16 * 16 + 16;
+                    for (uint32_t o = threadIdx.x * 16; o < (filled < pitch ? filled : pitch); o += THREADS * 16) {
                         if (o == 0 && row == 0 && ld != 0) {
                             for (uint32_t b = ld; b < 16 && b < bytes; b += sizeof(T))
                                 *reinterpret_cast<T*>(at(slot, t) + b) = *reinterpret_cast<const T*>(a + b);
                         } else {
-                            cp_async16(sm100::smem_u32(at(slot, t) + o), a + o, bytes - o < 16 ? bytes - o : 16);
+                            // (a block of zeros reads nothing; its address is the row's)
+                            const uint32_t n = o >= bytes ? 0 : bytes - o < 16 ? bytes - o : 16;
+                            cp_async16(sm100::smem_u32(at(slot, t) + o), n ? a + o : a, n);
                         }
                     }
                 }
@@ -337,6 +347,7 @@ template <typename T, bool VEC, int THREADS, int NT> struct Ring {
     template <typename C> __device__ __forceinline__ void start(const C& cl) {
         for (uint32_t s = 0; s < stages; ++s)
             for (int t = 0; t < NT; ++t) cl.pad(at(s, t));
+        if constexpr (!VEC) __syncthreads();
         for (uint32_t s = 1; s < stages; ++s) issue();
     }
 };
