@@ -104,13 +104,74 @@ enum Mode : int {
 
 struct PairParams {
     int M, N;              // rows and columns of an output (FORWARD: columns of out)
-    int m_tiles, n_tiles, tiles, total_tiles;  // tiles: of one output
+    int m_tiles, n_tiles, tiles;  // tiles: of one output
+    // Work items: `whole` tiles, then the remaining tiles, too few for one each per CTA pair, cut along K into
+    // `cuts` items each, whose fp32 sums go to part[item][column / 4][row] for a second kernel to join in order.
+    int items, whole, cuts;
+    float4* part;
     int num_kb, half_kb;   // K blocks in all, and of the first half (DX)
     long long ldc;
     uint16_t* out[3];      // FORWARD: out, g, u (the last two may be null); DX: dx; DW: dWg, dWu
     int vec, f16, act;
     int a_second;          // DW: which operand differs between dWg and dWu (1: A, 0: B)
 };
+
+struct PairItem {
+    int which, mb, nb;  // the output, and its tile
+    int kb0, kbs;       // first K block and number of them
+    int part;           // index of the partial sum, -1 for a whole tile
+};
+
+// First K block (or end, for cut + 1) of a cut tile's part.
+__device__ __forceinline__ int cut_begin(const PairParams& p, int cut) {
+    return static_cast<int>(static_cast<long long>(p.num_kb) * cut / p.cuts);
+}
+
+template <int MODE> __device__ __forceinline__ PairItem pair_item(const PairParams& p, int item) {
+    PairItem w;
+    int tile = item;
+    w.kb0 = 0;
+    w.kbs = p.num_kb;
+    w.part = -1;
+    if (item >= p.whole) {
+        w.part = item - p.whole;
+        tile = p.whole + w.part / p.cuts;
+        const int cut = w.part % p.cuts;
+        w.kb0 = cut_begin(p, cut);
+        w.kbs = cut_begin(p, cut + 1) - w.kb0;
+    }
+    w.which = MODE == DW ? tile / p.tiles : 0;
+    grouped_tile(tile - w.which * p.tiles, p.m_tiles, p.n_tiles, w.mb, w.nb);
+    return w;
+}
+
+// Columns c * 32 to c * 32 + 31 of a tile's row (FORWARD: rg of g and ru of u, else rg alone), to the outputs.
+template <int MODE>
+__device__ __forceinline__ void store_tile_row(const PairParams& p, const PairItem& w, int row, int c, const uint32_t (&rg)[32],
+                                               const uint32_t (&ru)[32]) {
+    constexpr int WIDTH = MODE == FORWARD ? 128 : 256;
+    const int col = w.nb * WIDTH + c * 32, n = p.N - col;
+    if (row >= p.M || n <= 0) return;
+    const long long o = static_cast<long long>(row) * p.ldc + col;
+    float v[32];
+    if constexpr (MODE == FORWARD) {
+        if (p.out[1]) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rg[j]);
+            store32(p.out[1] + o, v, n, p.vec, p.f16);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(ru[j]);
+            store32(p.out[2] + o, v, n, p.vec, p.f16);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = activation(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
+        store32(p.out[0] + o, v, n, p.vec, p.f16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rg[j]);
+        store32((MODE == DW && w.which ? p.out[1] : p.out[0]) + o, v, n, p.vec, p.f16);
+    }
+}
 
 // 256 x 256 accumulators (FORWARD: 128 columns of g and 128 of u), BK = 128 per
 // stage in boxes of 16 KiB, three stages; two accumulators in TMEM so that a
@@ -174,22 +235,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_sh;
 
-    // which output, and its tile's coordinates
-    auto coords = [&](int tile, int& which, int& mb, int& nb) {
-        which = MODE == DW ? tile / p.tiles : 0;
-        grouped_tile(tile - which * p.tiles, p.m_tiles, p.n_tiles, mb, nb);
-    };
-
     if (warp == 0) {
         // ------------------------------------------------ TMA producer (both CTAs)
         int stage = 0;
         uint32_t phase = 0;
         long long issued = 0;
-        for (int tile = pair; tile < p.total_tiles; tile += npairs) {
+        for (int item = pair; item < p.items; item += npairs) {
             if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-            int which, mb, nb;
-            coords(tile, which, mb, nb);
-            for (int kb = 0; kb < p.num_kb; ++kb) {
+            const PairItem w = pair_item<MODE>(p, item);
+            for (int kb = 0; kb < w.kbs; ++kb) {
                 bool ok = true;
                 if (lane == 0) ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, status, 31);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -199,7 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                     uint8_t* sb = sa + 2 * Cfg::BOX;
                     const uint32_t full_leader = mapa_shared(smem_u32(&full_bar[stage]), 0);
                     if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE);
-                    int k = k_block(kb, tile / npairs, p.num_kb);
+                    int k = w.kb0 + k_block(kb, item / npairs, w.kbs);
                     bool second_a = false, second_b = false;
                     if (MODE == FORWARD) {
                         second_b = !leader;
@@ -207,13 +261,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                         second_a = second_b = k >= p.half_kb;
                         if (second_a) k -= p.half_kb;
                     } else {
-                        second_a = which != 0 && p.a_second;
-                        second_b = which != 0 && !p.a_second;
+                        second_a = w.which != 0 && p.a_second;
+                        second_b = w.which != 0 && !p.a_second;
                     }
                     const CUtensorMap* ta = second_a ? &tmA1 : &tmA0;
                     const CUtensorMap* tb = second_b ? &tmB1 : &tmB0;
-                    const int m0 = mb * Cfg::BM + static_cast<int>(rank) * 128;
-                    const int n0 = MODE == FORWARD ? nb * 128 : nb * Cfg::BN + static_cast<int>(rank) * 128;
+                    const int m0 = w.mb * Cfg::BM + static_cast<int>(rank) * 128;
+                    const int n0 = MODE == FORWARD ? w.nb * 128 : w.nb * Cfg::BN + static_cast<int>(rank) * 128;
                     const int k0 = k * Cfg::BK;
                     if constexpr (A_MN) {
                         tma_load_3d_pair(sa, ta, full_leader, m0, k0, 0);
@@ -254,8 +308,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             uint32_t phase = 0;
             int local = 0;
             bool issued_any = false;
-            for (int tile = pair; tile < p.total_tiles; tile += npairs, ++local) {
+            for (int item = pair; item < p.items; item += npairs, ++local) {
                 if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+                const int cut = item < p.whole ? 0 : (item - p.whole) % p.cuts;
+                const int kbs = item < p.whole ? p.num_kb : cut_begin(p, cut + 1) - cut_begin(p, cut);
                 const int acc = local & 1;
                 const uint32_t acc_phase = static_cast<uint32_t>((local >> 1) & 1);
                 bool ok = true;
@@ -264,7 +320,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * Cfg::BN);
-                for (int kb = 0; kb < p.num_kb; ++kb) {
+                for (int kb = 0; kb < kbs; ++kb) {
                     if (lane == 0) ok = mbar_wait(&full_bar[stage], phase, abort_flag, status, 34);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
                     if (!ok) break;
@@ -306,58 +362,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         const uint32_t tempty_leader0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
         const uint32_t tempty_leader1 = mapa_shared(smem_u32(&tempty_bar[1]), 0);
         int local = 0;
-        for (int tile = pair; tile < p.total_tiles; tile += npairs, ++local) {
+        for (int item = pair; item < p.items; item += npairs, ++local) {
             if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-            int which, mb, nb;
-            coords(tile, which, mb, nb);
+            const PairItem w = pair_item<MODE>(p, item);
             const int acc = local & 1;
             const uint32_t acc_phase = static_cast<uint32_t>((local >> 1) & 1);
             bool ok = mbar_wait(&tfull_bar[acc], acc_phase, abort_flag, status, 36);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            const int row = mb * Cfg::BM + static_cast<int>(rank) * 128 + q * 32 + lane;
-            const long long row_off = static_cast<long long>(row) * p.ldc;
+            const int tile_row = static_cast<int>(rank) * 128 + q * 32 + lane;
             const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * Cfg::BN) + (static_cast<uint32_t>(q * 32) << 16);
-            if constexpr (MODE == FORWARD) {
+            constexpr int STEP = MODE == FORWARD ? 128 : Cfg::BN;  // FORWARD: u is 128 columns after g
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t rg[32], ru[32];
-                    tmem_ld_32x32b_x32(taddr + c * 32, rg);
-                    tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
-                    tmem_ld_wait();
-                    const int col = nb * 128 + c * 32, n = p.N - col;
-                    if (row < p.M && n > 0) {
-                        float v[32];
-                        if (p.out[1]) {
+            for (int c = 0; c < STEP / 32; ++c) {
+                uint32_t rg[32], ru[32];
+                tmem_ld_32x32b_x32(taddr + c * 32, rg);
+                if (MODE == FORWARD) tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
+                tmem_ld_wait();
+                if (w.part < 0) {
+                    store_tile_row<MODE>(p, w, w.mb * Cfg::BM + tile_row, c, rg, ru);
+                } else {
+                    float4* part = p.part + static_cast<size_t>(w.part) * (Cfg::BM * Cfg::BN / 4) + tile_row;
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rg[j]);
-                            store32(p.out[1] + row_off + col, v, n, p.vec, p.f16);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(ru[j]);
-                            store32(p.out[2] + row_off + col, v, n, p.vec, p.f16);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = activation(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
-                        store32(p.out[0] + row_off + col, v, n, p.vec, p.f16);
+                    for (int v = 0; v < 8; ++v) {
+                        part[(c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(rg[4 * v]), __uint_as_float(rg[4 * v + 1]),
+                                                                  __uint_as_float(rg[4 * v + 2]), __uint_as_float(rg[4 * v + 3]));
+                        if (MODE == FORWARD)
+                            part[(32 + c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(ru[4 * v]), __uint_as_float(ru[4 * v + 1]),
+                                                                           __uint_as_float(ru[4 * v + 2]), __uint_as_float(ru[4 * v + 3]));
                     }
-                    __syncwarp();  // the next TMEM load is a warp-wide instruction
                 }
-            } else {
-                uint16_t* out = MODE == DW && which ? p.out[1] : p.out[0];
-#pragma unroll 1
-                for (int c = 0; c < Cfg::BN / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(taddr + c * 32, r);
-                    tmem_ld_wait();
-                    const int col = nb * Cfg::BN + c * 32, n = p.N - col;
-                    if (row < p.M && n > 0) {
-                        float v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                        store32(out + row_off + col, v, n, p.vec, p.f16);
-                    }
-                    __syncwarp();
-                }
+                __syncwarp();  // the next TMEM load is a warp-wide instruction
             }
             tc_fence_before();
             __syncwarp();
@@ -370,6 +405,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     cluster_sync();  // no CTA leaves while its peer may still touch its barriers or shared memory
     tc_fence_after();
     if (warp == 1) tmem_dealloc_pair<Cfg::TMEM_COLS>(tmem_base);
+}
+
+// Joins the cut tiles: block (t, c) adds the partial sums of columns c * 32 to c * 32 + 31
+// (FORWARD: of g and of u) of tile `whole` + t, a row per thread, and stores the results.
+template <int MODE> __global__ void __launch_bounds__(256) gated_pair_join_kernel(const PairParams p) {
+    pdl_wait();
+    const int first = blockIdx.x * p.cuts, c = blockIdx.y;
+    const PairItem w = pair_item<MODE>(p, p.whole + first);
+    uint32_t rg[32], ru[32];
+    float4 g[8], u[8];
+#pragma unroll
+    for (int v = 0; v < 8; ++v) g[v] = u[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < p.cuts; ++i) {
+        const float4* part = p.part + static_cast<size_t>(first + i) * (PairCfg::BM * PairCfg::BN / 4) + threadIdx.x;
+#pragma unroll
+        for (int v = 0; v < 8; ++v) {
+            const float4 a = part[(c * 8 + v) * PairCfg::BM];
+            g[v].x += a.x; g[v].y += a.y; g[v].z += a.z; g[v].w += a.w;
+            if (MODE == FORWARD) {
+                const float4 b = part[(32 + c * 8 + v) * PairCfg::BM];
+                u[v].x += b.x; u[v].y += b.y; u[v].z += b.z; u[v].w += b.w;
+            }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+        rg[4 * v] = __float_as_uint(g[v].x); rg[4 * v + 1] = __float_as_uint(g[v].y);
+        rg[4 * v + 2] = __float_as_uint(g[v].z); rg[4 * v + 3] = __float_as_uint(g[v].w);
+        ru[4 * v] = __float_as_uint(u[v].x); ru[4 * v + 1] = __float_as_uint(u[v].y);
+        ru[4 * v + 2] = __float_as_uint(u[v].z); ru[4 * v + 3] = __float_as_uint(u[v].w);
+    }
+    store_tile_row<MODE>(p, w, w.mb * PairCfg::BM + static_cast<int>(threadIdx.x), c, rg, ru);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -693,13 +760,31 @@ int launch_pair(const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, Pair
     const long long tiles = static_cast<long long>(p.m_tiles) * p.n_tiles, total = tiles * (MODE == DW ? 2 : 1);
     if (total > 0x3fffffff) return fail(cudaErrorInvalidValue, "%s: too many output tiles", what);
     p.tiles = static_cast<int>(tiles);
-    p.total_tiles = static_cast<int>(total);
+    // The tiles after the last full round of the pairs are cut along K, so that the round they take is as short as
+    // the pairs allow: up to 8 cuts of at least 8 K blocks each (the join costs about 5 us).
+    const int pairs = sm_count() / 2, rest = static_cast<int>(total % pairs);
+    p.cuts = 1;
+    while (rest > 0 && p.cuts < 8 && rest * (p.cuts + 1) <= pairs && p.num_kb >= 8 * (p.cuts + 1)) ++p.cuts;
+    p.whole = static_cast<int>(total) - (p.cuts > 1 ? rest : 0);
+    p.items = p.cuts > 1 ? p.whole + rest * p.cuts : p.whole;
+    Scratch parts{nullptr, 0, st, what};
+    if (p.cuts > 1) {
+        if (int rc = parts.open(static_cast<size_t>(rest * p.cuts) * Cfg::BM * Cfg::BN * sizeof(float))) return rc;
+        p.part = reinterpret_cast<float4*>(parts.base);
+    }
     auto gated_pair = gated_pair_kernel<MODE, A_MN, B_MN>;
     static SmemLimit limit;
-    if (int rc = limit.ensure(gated_pair, Cfg::SMEM, what)) return rc;
-    const int pairs = sm_count() / 2;
-    gated_pair<<<2 * (p.total_tiles < pairs ? p.total_tiles : pairs), 192, Cfg::SMEM, st>>>(ta0, ta1, tb0, tb1, p);
-    return launch_status(what);
+    int rc = limit.ensure(gated_pair, Cfg::SMEM, what);
+    if (rc == 0) {
+        gated_pair<<<2 * (p.items < pairs ? p.items : pairs), 192, Cfg::SMEM, st>>>(ta0, ta1, tb0, tb1, p);
+        rc = launch_status(what);
+    }
+    if (rc == 0 && p.cuts > 1) {
+        const dim3 grid(static_cast<unsigned>(rest), MODE == FORWARD ? 4 : 8);
+        launch_pdl(gated_pair_join_kernel<MODE>, grid, 256, 0, st, p);
+        rc = launch_status(what);
+    }
+    return parts.close(rc);
 }
 
 // 128 rows: 66.8 us there, 64 as one tile of the pair kernel (4096 -> 14336)

@@ -113,9 +113,10 @@ def check_backward(torch, x, wg, wu, g, u, dout, act, trans, extra=0):
 
 # rows around each padding of the few-rows kernel, its border, and the 256-row tiles; columns below, at and past the
 # 128-column tile; contractions of less than one block, odd counts of blocks, and cut by clusters
+# or over the last round of pairs (after whole rounds and without any)
 SHAPES = [(1, 8, 8), (1, 64, 128), (2, 200, 136), (16, 512, 264), (17, 1000, 128), (32, 4096, 256), (33, 72, 520), (64, 2048, 1032),
           (65, 640, 384), (128, 1096, 392), (129, 512, 256), (255, 128, 136), (256, 384, 128), (257, 1000, 776), (520, 2056, 640),
-          (1000, 264, 2048)]
+          (1000, 264, 2048), (300, 4096, 520), (66, 2056, 1000), (2600, 2048, 1032), (2100, 520, 264)]
 
 
 @pytest.mark.parametrize("trans", [False, True])
