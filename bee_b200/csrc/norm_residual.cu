@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
     uint32_t slot = 0;
     float rh = 1.f;  // of the current row; found with the sums of the row before
     ring.advance();
-    if (wpost) rh = rsqrtf(fmaf(block_sum(squares(ring.read(0, 0, r0))), inv_n, a.eps));
+    // (as the second of two sums, like every other row's: a row's results do not depend on the rows around it)
+    if (wpost) rh = rsqrtf(fmaf(block_sum(0.f, squares(ring.read(0, 0, r0))).y, inv_n, a.eps));
     for (long long r = r0; r < r1; ++r) {
         f2 hh[kPairs], v[kPairs], w[kPairs], t[kPairs];
         // hh = h rstd(h), v = x'
