@@ -74,6 +74,21 @@ __device__ __forceinline__ void activation_grad(float g, int act, float& a, floa
     }
 }
 
+// g = act(g) u for N columns in registers (bits of fp32).  One loop per activation: with the choice inside, the
+// unrolled code of all three outgrows the instruction cache (1024 x 1024 -> 4096: 47 us against 25).
+template <int N> __device__ __forceinline__ void gate_columns(uint32_t (&g)[N], const uint32_t (&u)[N], int act) {
+    if (act == ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) g[j] = __float_as_uint(activation(__uint_as_float(g[j]), ACT_SILU) * __uint_as_float(u[j]));
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) g[j] = __float_as_uint(activation(__uint_as_float(g[j]), ACT_GELU) * __uint_as_float(u[j]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) g[j] = __float_as_uint(activation(__uint_as_float(g[j]), ACT_GELU_TANH) * __uint_as_float(u[j]));
+    }
+}
+
 __device__ __forceinline__ uint32_t pack16(float lo, float hi, int f16) { return f16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi); }
 __device__ __forceinline__ uint16_t round16(float v, int f16) { return static_cast<uint16_t>(pack16(v, 0.f, f16) & 0xffffu); }
 __device__ __forceinline__ float up16(uint16_t v, int f16) {
@@ -147,7 +162,7 @@ template <int MODE> __device__ __forceinline__ PairItem pair_item(const PairPara
 
 // Columns c * 32 to c * 32 + 31 of a tile's row (FORWARD: rg of g and ru of u, else rg alone), to the outputs.
 template <int MODE>
-__device__ __forceinline__ void store_tile_row(const PairParams& p, const PairItem& w, int row, int c, const uint32_t (&rg)[32],
+__device__ __forceinline__ void store_tile_row(const PairParams& p, const PairItem& w, int row, int c, uint32_t (&rg)[32],
                                                const uint32_t (&ru)[32]) {
     constexpr int WIDTH = MODE == FORWARD ? 128 : 256;
     const int col = w.nb * WIDTH + c * 32, n = p.N - col;
@@ -163,8 +178,9 @@ __device__ __forceinline__ void store_tile_row(const PairParams& p, const PairIt
             for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(ru[j]);
             store32(p.out[2] + o, v, n, p.vec, p.f16);
         }
+        gate_columns(rg, ru, p.act);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = activation(__uint_as_float(rg[j]), p.act) * __uint_as_float(ru[j]);
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(rg[j]);
         store32(p.out[0] + o, v, n, p.vec, p.f16);
     } else {
 #pragma unroll
@@ -181,14 +197,38 @@ struct PairCfg {
     static constexpr int BOX = 128 * 64 * 2;
     static constexpr int STAGE = 4 * BOX;  // this CTA's 128 rows of A and 128 columns of B
     static constexpr int STAGES = 3;
-    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int OUT = 32 * 64 * 2;  // an epilogue warp's 32 rows of 64 output columns, as TMA stores them
+    static constexpr int SMEM = STAGES * STAGE + 4 * 2 * OUT + 1024;
     static constexpr uint32_t TMEM_COLS = 512;
 };
+
+// One epilogue warp's 32 rows x 64 columns: rounded into its next staging buffer (128-byte rows, swizzled as the map
+// says) and stored by TMA, which cuts what lies outside the output.  v(j): the lane's row's column j.
+template <typename V>
+__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* stage, int& turn, int lane, int row0, int col, int f16, V v) {
+    if (lane == 0) tma_store_wait_read_all_but<1>();  // the buffer's last store has been read
+    __syncwarp();
+    uint8_t* row = stage + turn * PairCfg::OUT + lane * 128;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(row + ((c ^ (lane & 7)) << 4)) =
+            make_uint4(pack16(v(8 * c), v(8 * c + 1), f16), pack16(v(8 * c + 2), v(8 * c + 3), f16),
+                       pack16(v(8 * c + 4), v(8 * c + 5), f16), pack16(v(8 * c + 6), v(8 * c + 7), f16));
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+        tma_store_3d(map, stage + turn * PairCfg::OUT, col, row0, 0);
+        tma_store_commit();
+    }
+    turn ^= 1;
+}
 
 template <int MODE, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     gated_pair_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
-                      const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1, const PairParams p) {
+                      const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                      const __grid_constant__ CUtensorMap tmO0, const __grid_constant__ CUtensorMap tmO1,
+                      const __grid_constant__ CUtensorMap tmO2, const PairParams p) {
     using Cfg = PairCfg;
     constexpr int STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
@@ -361,6 +401,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
         const int q = warp & 3;
         const uint32_t tempty_leader0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
         const uint32_t tempty_leader1 = mapa_shared(smem_u32(&tempty_bar[1]), 0);
+        uint8_t* out_stage = smem + STAGES * Cfg::STAGE + q * 2 * Cfg::OUT;
+        int out_turn = 0;
         int local = 0;
         for (int item = pair; item < p.items; item += npairs, ++local) {
             if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
@@ -373,31 +415,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             const int tile_row = static_cast<int>(rank) * 128 + q * 32 + lane;
             const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * Cfg::BN) + (static_cast<uint32_t>(q * 32) << 16);
             constexpr int STEP = MODE == FORWARD ? 128 : Cfg::BN;  // FORWARD: u is 128 columns after g
+            const int row0 = w.mb * Cfg::BM + tile_row - lane;
+            if (w.part < 0 && p.vec) {
 #pragma unroll 1
-            for (int c = 0; c < STEP / 32; ++c) {
-                uint32_t rg[32], ru[32];
-                tmem_ld_32x32b_x32(taddr + c * 32, rg);
-                if (MODE == FORWARD) tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
-                tmem_ld_wait();
-                if (w.part < 0) {
-                    store_tile_row<MODE>(p, w, w.mb * Cfg::BM + tile_row, c, rg, ru);
-                } else {
-                    float4* part = p.part + static_cast<size_t>(w.part) * (Cfg::BM * Cfg::BN / 4) + tile_row;
-#pragma unroll
-                    for (int v = 0; v < 8; ++v) {
-                        part[(c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(rg[4 * v]), __uint_as_float(rg[4 * v + 1]),
-                                                                  __uint_as_float(rg[4 * v + 2]), __uint_as_float(rg[4 * v + 3]));
-                        if (MODE == FORWARD)
-                            part[(32 + c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(ru[4 * v]), __uint_as_float(ru[4 * v + 1]),
-                                                                           __uint_as_float(ru[4 * v + 2]), __uint_as_float(ru[4 * v + 3]));
+                for (int c = 0; c < STEP; c += 64) {
+                    uint32_t g0[32], g1[32], u0[32], u1[32];
+                    tmem_ld_32x32b_x32(taddr + c, g0);
+                    tmem_ld_32x32b_x32(taddr + c + 32, g1);
+                    if (MODE == FORWARD) {
+                        tmem_ld_32x32b_x32(taddr + 128 + c, u0);
+                        tmem_ld_32x32b_x32(taddr + 128 + c + 32, u1);
                     }
+                    tmem_ld_wait();
+                    const int col = w.nb * STEP + c;
+                    if (row0 < p.M && col < p.N) {
+                        auto g = [&](int j) { return __uint_as_float(j < 32 ? g0[j & 31] : g1[j & 31]); };
+                        auto u = [&](int j) { return __uint_as_float(j < 32 ? u0[j & 31] : u1[j & 31]); };
+                        if constexpr (MODE == FORWARD) {
+                            if (p.out[1]) {
+                                store_block(&tmO1, out_stage, out_turn, lane, row0, col, p.f16, g);
+                                store_block(&tmO2, out_stage, out_turn, lane, row0, col, p.f16, u);
+                            }
+                            gate_columns(g0, u0, p.act);
+                            gate_columns(g1, u1, p.act);
+                            store_block(&tmO0, out_stage, out_turn, lane, row0, col, p.f16, g);
+                        } else {
+                            store_block(MODE == DW && w.which ? &tmO1 : &tmO0, out_stage, out_turn, lane, row0, col, p.f16, g);
+                        }
+                    }
+                    __syncwarp();  // the next TMEM load is a warp-wide instruction
                 }
-                __syncwarp();  // the next TMEM load is a warp-wide instruction
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < STEP / 32; ++c) {
+                    uint32_t rg[32], ru[32];
+                    tmem_ld_32x32b_x32(taddr + c * 32, rg);
+                    if (MODE == FORWARD) tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
+                    tmem_ld_wait();
+                    if (w.part < 0) {
+                        store_tile_row<MODE>(p, w, w.mb * Cfg::BM + tile_row, c, rg, ru);
+                    } else {
+                        float4* part = p.part + static_cast<size_t>(w.part) * (Cfg::BM * Cfg::BN / 4) + tile_row;
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) {
+                            part[(c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(rg[4 * v]), __uint_as_float(rg[4 * v + 1]),
+                                                                      __uint_as_float(rg[4 * v + 2]), __uint_as_float(rg[4 * v + 3]));
+                            if (MODE == FORWARD)
+                                part[(32 + c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(ru[4 * v]), __uint_as_float(ru[4 * v + 1]),
+                                                                               __uint_as_float(ru[4 * v + 2]), __uint_as_float(ru[4 * v + 3]));
+                        }
+                    }
+                    __syncwarp();
+                }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc ? tempty_leader1 : tempty_leader0);
         }
+        if (lane == 0) tma_store_wait_read();  // the staging buffers must outlive their stores
+        __syncwarp();
     }
 
     tc_fence_before();
@@ -754,6 +830,12 @@ int launch_pair(const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, Pair
     if (int rc = map_of(&ta1, a1, 128, f16)) return rc;
     if (int rc = map_of(&tb0, b0, 128, f16)) return rc;
     if (int rc = map_of(&tb1, b1, 128, f16)) return rc;
+    CUtensorMap to[3] = {ta0, ta0, ta0};  // of the outputs, where TMA can store them (p.vec)
+    for (int i = 0; i < 3; ++i) {
+        if (!p.vec || !p.out[i]) continue;
+        const Mat o{p.out[i], p.M, p.N, p.ldc};
+        if (int rc = map_of(&to[i], o, 32, f16)) return rc;
+    }
     const int bn = MODE == FORWARD ? 128 : Cfg::BN;
     p.m_tiles = (p.M + Cfg::BM - 1) / Cfg::BM;
     p.n_tiles = (p.N + bn - 1) / bn;
@@ -776,7 +858,7 @@ int launch_pair(const Mat& a0, const Mat& a1, const Mat& b0, const Mat& b1, Pair
     static SmemLimit limit;
     int rc = limit.ensure(gated_pair, Cfg::SMEM, what);
     if (rc == 0) {
-        gated_pair<<<2 * (p.items < pairs ? p.items : pairs), 192, Cfg::SMEM, st>>>(ta0, ta1, tb0, tb1, p);
+        gated_pair<<<2 * (p.items < pairs ? p.items : pairs), 192, Cfg::SMEM, st>>>(ta0, ta1, tb0, tb1, to[0], to[1], to[2], p);
         rc = launch_status(what);
     }
     if (rc == 0 && p.cuts > 1) {
