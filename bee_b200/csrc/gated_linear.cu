@@ -203,22 +203,37 @@ struct PairCfg {
 };
 
 // One epilogue warp's 32 rows x 64 columns: rounded into its next staging buffer (128-byte rows, swizzled as the map
-// says) and stored by TMA, which cuts what lies outside the output.  v(j): the lane's row's column j.
+// says) and stored by TMA, which cuts what lies outside the output; outputs that TMA cannot describe (odd strides) are
+// written from the buffer row by row, a column per lane.  v(j): the lane's row's column j.
 template <typename V>
-__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* stage, int& turn, int lane, int row0, int col, int f16, V v) {
+__device__ __forceinline__ void store_block(const PairParams& p, const CUtensorMap* map, uint16_t* out, uint8_t* stage, int& turn, int lane,
+                                            int row0, int col, V v) {
     if (lane == 0) tma_store_wait_read_all_but<1>();  // the buffer's last store has been read
     __syncwarp();
-    uint8_t* row = stage + turn * PairCfg::OUT + lane * 128;
+    uint8_t* block = stage + turn * PairCfg::OUT;
 #pragma unroll
     for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<uint4*>(row + ((c ^ (lane & 7)) << 4)) =
-            make_uint4(pack16(v(8 * c), v(8 * c + 1), f16), pack16(v(8 * c + 2), v(8 * c + 3), f16),
-                       pack16(v(8 * c + 4), v(8 * c + 5), f16), pack16(v(8 * c + 6), v(8 * c + 7), f16));
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-        tma_store_3d(map, stage + turn * PairCfg::OUT, col, row0, 0);
-        tma_store_commit();
+        *reinterpret_cast<uint4*>(block + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+            make_uint4(pack16(v(8 * c), v(8 * c + 1), p.f16), pack16(v(8 * c + 2), v(8 * c + 3), p.f16),
+                       pack16(v(8 * c + 4), v(8 * c + 5), p.f16), pack16(v(8 * c + 6), v(8 * c + 7), p.f16));
+    if (p.vec) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_3d(map, block, col, row0, 0);
+            tma_store_commit();
+        }
+    } else {
+        __syncwarp();
+        const int rows = min(32, p.M - row0);
+        for (int r = 0; r < rows; ++r) {
+            uint16_t* dst = out + static_cast<long long>(row0 + r) * p.ldc + col;
+#pragma unroll
+            for (int j = lane; j < 64; j += 32) {
+                const uint16_t x = *reinterpret_cast<const uint16_t*>(block + r * 128 + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2);
+                if (col + j < p.N) dst[j] = x;
+            }
+        }
     }
     turn ^= 1;
 }
@@ -416,7 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
             const uint32_t taddr = tmem_base + static_cast<uint32_t>(acc * Cfg::BN) + (static_cast<uint32_t>(q * 32) << 16);
             constexpr int STEP = MODE == FORWARD ? 128 : Cfg::BN;  // FORWARD: u is 128 columns after g
             const int row0 = w.mb * Cfg::BM + tile_row - lane;
-            if (w.part < 0 && p.vec) {
+            if (w.part < 0) {
 #pragma unroll 1
                 for (int c = 0; c < STEP; c += 64) {
                     uint32_t g0[32], g1[32], u0[32], u1[32];
@@ -433,39 +448,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
                         auto u = [&](int j) { return __uint_as_float(j < 32 ? u0[j & 31] : u1[j & 31]); };
                         if constexpr (MODE == FORWARD) {
                             if (p.out[1]) {
-                                store_block(&tmO1, out_stage, out_turn, lane, row0, col, p.f16, g);
-                                store_block(&tmO2, out_stage, out_turn, lane, row0, col, p.f16, u);
+                                store_block(p, &tmO1, p.out[1], out_stage, out_turn, lane, row0, col, g);
+                                store_block(p, &tmO2, p.out[2], out_stage, out_turn, lane, row0, col, u);
                             }
                             gate_columns(g0, u0, p.act);
                             gate_columns(g1, u1, p.act);
-                            store_block(&tmO0, out_stage, out_turn, lane, row0, col, p.f16, g);
+                            store_block(p, &tmO0, p.out[0], out_stage, out_turn, lane, row0, col, g);
                         } else {
-                            store_block(MODE == DW && w.which ? &tmO1 : &tmO0, out_stage, out_turn, lane, row0, col, p.f16, g);
+                            const bool second = MODE == DW && w.which;
+                            store_block(p, second ? &tmO1 : &tmO0, second ? p.out[1] : p.out[0], out_stage, out_turn, lane, row0, col, g);
                         }
                     }
                     __syncwarp();  // the next TMEM load is a warp-wide instruction
                 }
             } else {
+                float4* part = p.part + static_cast<size_t>(w.part) * (Cfg::BM * Cfg::BN / 4) + tile_row;
 #pragma unroll 1
-                for (int c = 0; c < STEP / 32; ++c) {
-                    uint32_t rg[32], ru[32];
-                    tmem_ld_32x32b_x32(taddr + c * 32, rg);
-                    if (MODE == FORWARD) tmem_ld_32x32b_x32(taddr + 128 + c * 32, ru);
+                for (int c = 0; c < Cfg::BN / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(taddr + c * 32, r);
                     tmem_ld_wait();
-                    if (w.part < 0) {
-                        store_tile_row<MODE>(p, w, w.mb * Cfg::BM + tile_row, c, rg, ru);
-                    } else {
-                        float4* part = p.part + static_cast<size_t>(w.part) * (Cfg::BM * Cfg::BN / 4) + tile_row;
 #pragma unroll
-                        for (int v = 0; v < 8; ++v) {
-                            part[(c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(rg[4 * v]), __uint_as_float(rg[4 * v + 1]),
-                                                                      __uint_as_float(rg[4 * v + 2]), __uint_as_float(rg[4 * v + 3]));
-                            if (MODE == FORWARD)
-                                part[(32 + c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(ru[4 * v]), __uint_as_float(ru[4 * v + 1]),
-                                                                               __uint_as_float(ru[4 * v + 2]), __uint_as_float(ru[4 * v + 3]));
-                        }
-                    }
-                    __syncwarp();
+                    for (int v = 0; v < 8; ++v)
+                        part[(c * 8 + v) * Cfg::BM] = make_float4(__uint_as_float(r[4 * v]), __uint_as_float(r[4 * v + 1]),
+                                                                  __uint_as_float(r[4 * v + 2]), __uint_as_float(r[4 * v + 3]));
                 }
             }
             tc_fence_before();

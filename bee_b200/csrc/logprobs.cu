@@ -23,8 +23,9 @@
 // maxima do again (one or two of a thread, all of them if its third may), an element
 // per lane, and lists the elements that reach the bound; the rank of each among all is
 // counted.  Order is that of (value, ~index) keys of 64 bits: ties go to the lowest index.
-// Rows with more such elements than a list holds (many ties, or hardly anything
-// unmasked) insert them one by one into sorted lists instead.
+// Where fewer than k elements are unmasked, masked ones follow by index.  Rows with more
+// elements that reach the bound than a list holds (many ties) insert them one by one into
+// sorted lists instead.
 // This costs latency at the end of a row (4 rows of 131072 bf16: 4.5 us without
 // alternatives, 8.6 us with 20); sorting the group maxima and merging the warps' lists
 // took 1 to 4 us more, reading the whole shares of the threads concerned 2 to 10 us.
@@ -478,7 +479,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 n1 += (g.x > g1) + (g.y > g1) + (g.z > g1) + (g.w > g1);
             }
             const uint32_t o0 = n0 < a.top ? ordered(g0) : 0xffffffffu, o1 = n1 < a.top ? ordered(g1) : 0xffffffffu;
-            const float bound = from_ordered(__reduce_min_sync(0xffffffffu, o0 < o1 ? o0 : o1));
+            // (where fewer than k groups hold anything unmasked, every unmasked element is a candidate)
+            const float bound = fmaxf(from_ordered(__reduce_min_sync(0xffffffffu, o0 < o1 ? o0 : o1)), -3.402823466e+38f);
 
             // the warp's elements that reach it
             const int batches = whole + (rest > 0);
@@ -529,9 +531,28 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
             if (lane == 0) listed[warp] = held;
             __syncthreads();
             bool over = false;
+            int found = 0;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) over |= listed[w] > 32;
+            for (int w = 0; w < WARPS; ++w) {
+                over |= listed[w] > 32;
+                found += listed[w];
+            }
             if (!over) {
+                // fewer than k unmasked elements: masked ones follow by index, and fewer than k of the first 64 are not masked
+                if (warp == 0 && found < a.top) {
+                    const long long i0 = part.edge_lo >= 0 ? 0 : row.first(part.lo);
+                    const long long i1 = part.edge_hi >= 0 ? row.n : min(row.n, row.first(part.hi));
+                    int place = found;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const long long i = i0 + h * 32 + lane;
+                        const bool masked = i < i1 && Elems<T>::get(row.row + i) == -INFINITY;
+                        const uint32_t all = __ballot_sync(0xffffffffu, masked);
+                        const int at = place + __popc(all & ((1u << lane) - 1u));
+                        if (masked && at < a.top) sorted[at] = make_key(-INFINITY, static_cast<uint32_t>(i));
+                        place += __popc(all);
+                    }
+                }
                 if (lane < held) {
                     const uint64_t key = lists[warp][lane];
                     int place = 0;
