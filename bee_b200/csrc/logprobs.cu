@@ -529,15 +529,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 list(x[1], at[1]);
             }
             if (lane == 0) listed[warp] = held;
+            if (lane >= held) lists[warp][lane] = 0;
             __syncthreads();
-            bool over = false;
-            int found = 0;
+            int longest = 0, found = 0;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                over |= listed[w] > 32;
+                longest = max(longest, listed[w]);
                 found += listed[w];
             }
-            if (!over) {
+            if (longest <= 32) {
                 // fewer than k unmasked elements: masked ones follow by index, and fewer than k of the first 64 are not masked
                 if (warp == 0 && found < a.top) {
                     const long long i0 = part.edge_lo >= 0 ? 0 : row.first(part.lo);
@@ -555,13 +555,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
                 }
                 if (lane < held) {
                     const uint64_t key = lists[warp][lane];
-                    int place = 0;
-#pragma unroll 1
-                    for (int w = 0; w < WARPS; ++w) {
-                        const int n = listed[w];
-#pragma unroll 4
-                        for (int i = 0; i < n; ++i) place += lists[w][i] > key;
-                    }
+                    int place = 0;  // the keys above this one; the lists' ends are 0
+#pragma unroll 2
+                    for (int i = 0; i < longest; ++i)
+#pragma unroll
+                        for (int w = 0; w < WARPS; ++w) place += lists[w][i] > key;
                     if (place < a.top) sorted[place] = key;
                 }
             } else {
