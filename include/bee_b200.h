@@ -349,9 +349,10 @@ BEE_B200_API int bee_b200_bmm_strided(int dt_in, int dt_out, const void* A, int6
  * contiguous): x Wg and x Wu, kept for the backward.  act: 0 silu, 1 gelu (erf),
  * 2 gelu (tanh).  dt in {BF16, F16}; fp32 accumulation on the tensor cores, one
  * rounding per output (out from the unrounded products).  Up to 64 rows run a
- * kernel that is bound by reading the weights once.  Operands whose rows are not 16-byte
- * aligned are copied to padded scratch first (2 bytes an element of them, from
- * the stream-ordered pool). */
+ * kernel that is bound by reading the weights once.  Pool scratch, returned on the
+ * stream: operands whose rows are not 16-byte aligned are copied to padded
+ * rows first (2 bytes an element of them), and output tiles that are cut along the
+ * contraction leave fp32 partial sums (256 KiB for each of at most one per pair of SMs). */
 BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ldx, const void* wg, const void* wu,
                                        size_t ldw, int trans, void* out, void* g, void* u, size_t M, size_t D,
                                        size_t F, bee_b200_stream_t stream);
@@ -361,8 +362,8 @@ BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ld
  * dx = dg Wg^T + du Wu^T [M, D] contiguous; dwg = x^T dg and dwu = x^T du in the
  * weights' layout with row stride lddw.  dx may be NULL (then the weights are
  * not read), or dwg and dwu (then x is not).  Deterministic.  Takes 4*M*F bytes of
- * pool scratch (F rounded up to 8), plus the copies of unaligned operands as above.  Without rows
- * dwg and dwu are zeros. */
+ * pool scratch (F rounded up to 8), plus copies and partial sums as above.  Without
+ * rows dwg and dwu are zeros. */
 BEE_B200_API int bee_b200_gated_linear_backward(int dt, int act, const void* x, size_t ldx, const void* wg,
                                                 const void* wu, size_t ldw, int trans, const void* g, const void* u,
                                                 const void* dout, void* dx, void* dwg, void* dwu, size_t lddw,
