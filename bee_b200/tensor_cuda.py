@@ -339,6 +339,13 @@ def _pair(op: str, names: str, a: torch.Tensor, b: torch.Tensor, shape, dtype) -
     return ld
 
 
+def _width(op: str, name: str, t) -> int:
+    """Columns of a matrix that has to be given."""
+    if t is None or t.dim() != 2:
+        raise BeeError(op, 1, f"{name} must be 2-D")
+    return t.shape[1]
+
+
 def _matrix(op: str, name: str, t, m: int, n: int, dtype) -> int:
     """Pointer of an optional contiguous [m, n] matrix."""
     if t is None:
@@ -358,7 +365,7 @@ def gated_linear(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, out: torch
     _current(op, x, wg, wu, out, g, u)
     ldx = _rows(op, "x", x)
     m, d = x.shape
-    f = out.shape[-1]
+    f = _width(op, "out", out)
     ldw = _pair(op, "wg and wu", wg, wu, (f, d) if trans else (d, f), x.dtype)
     if (g is None) != (u is None):
         raise BeeError(op, 1, "g and u go together")
@@ -378,7 +385,7 @@ def gated_linear_backward(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, g
     _current(op, x, wg, wu, g, u, dout, dx, dwg, dwu)
     ldx = _rows(op, "x", x)
     m, d = x.shape
-    f = g.shape[-1]
+    f = _width(op, "g", g)
     shape = (f, d) if trans else (d, f)
     ldw = _pair(op, "wg and wu", wg, wu, shape, x.dtype)
     if (dwg is None) != (dwu is None):

@@ -129,3 +129,17 @@ def test_gated_backward_refusals(change):
 def test_gated_backward_stride():
     assert "stride" in refused(*gated_backward(lddw=95))
     accepted(*gated_backward(M=0, dwg=None, dwu=None, x=None, wg=None, wu=None, g=None, u=None, dout=None))
+
+
+def test_gated_wrappers_refuse_what_is_no_matrix(monkeypatch):
+    torch = pytest.importorskip("torch")
+    from bee_b200 import tensor_cuda as tc
+    monkeypatch.setattr(tc, "_current", lambda *a: None)  # the shapes are looked at on the host
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    for bad in (x[0, 0], x[0], x[None]):
+        with pytest.raises(tc.BeeError):
+            tc.gated_linear(x, x, x, bad)
+        with pytest.raises(tc.BeeError):
+            tc.gated_linear_backward(x, x, x, bad, x, x, dx=x)
+    with pytest.raises(tc.BeeError):
+        tc.gated_linear_backward(x, x, x, None, None, x, dx=x)
