@@ -934,6 +934,9 @@ int check(const char* what, int dt, int act, size_t M, size_t D, size_t F, size_
     return 0;
 }
 
+// Whether the output o, if there is one, is any of the tensors given.
+template <typename... P> bool is_any(const void* o, const P*... p) { return o && ((static_cast<const void*>(p) == o) || ...); }
+
 template <typename... P> bool aligned2(const P*... p) { return (((reinterpret_cast<uintptr_t>(p)) | ...) & 1u) == 0; }
 
 }  // namespace
@@ -958,6 +961,8 @@ int bee_b200_gated_linear(int dt, int act, const void* x, size_t ldx, const void
     if (M == 0) return ok();
     if (!x || !wg || !wu || !out || !g != !u) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
     if (!aligned2(x, wg, wu, out, g, u)) return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    if (is_any(out, x, wg, wu, g, u) || is_any(g, x, wg, wu, u) || is_any(u, x, wg, wu))
+        return fail(cudaErrorInvalidValue, "%s: outputs must not overlap the inputs or each other", what);
     cudaStream_t st = as_stream(stream);
     const long long m = static_cast<long long>(M), d = static_cast<long long>(D), f = static_cast<long long>(F);
     const long long lw = static_cast<long long>(ldw);
@@ -1014,6 +1019,8 @@ int bee_b200_gated_linear_backward(int dt, int act, const void* x, size_t ldx, c
     }
     if (!g || !u || !dout || (dx && (!wg || !wu)) || (dwg && !x)) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
     if (!aligned2(x, wg, wu, g, u, dout, dx, dwg, dwu)) return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    if (is_any(dx, x, wg, wu, dwg, dwu) || is_any(dwg, x, wg, wu, dwu) || is_any(dwu, x, wg, wu))
+        return fail(cudaErrorInvalidValue, "%s: gradients must not overlap the inputs or each other", what);
     const long long m = static_cast<long long>(M), d = static_cast<long long>(D), f = static_cast<long long>(F);
     const long long lw = static_cast<long long>(ldw);
     Mat mx{x, m, d, static_cast<long long>(ldx)};

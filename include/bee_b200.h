@@ -352,7 +352,8 @@ BEE_B200_API int bee_b200_bmm_strided(int dt_in, int dt_out, const void* A, int6
  * kernel that is bound by reading the weights once.  Pool scratch, returned on the
  * stream: operands whose rows are not 16-byte aligned are copied to padded
  * rows first (2 bytes an element of them), and output tiles that are cut along the
- * contraction leave fp32 partial sums (256 KiB for each of at most one per pair of SMs). */
+ * contraction leave fp32 partial sums (256 KiB for each of at most one per pair of SMs).  Outputs must not
+ * overlap the inputs or each other. */
 BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ldx, const void* wg, const void* wu,
                                        size_t ldw, int trans, void* out, void* g, void* u, size_t M, size_t D,
                                        size_t F, bee_b200_stream_t stream);
@@ -362,8 +363,8 @@ BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ld
  * dx = dg Wg^T + du Wu^T [M, D] contiguous; dwg = x^T dg and dwu = x^T du in the
  * weights' layout with row stride lddw.  dx may be NULL (then the weights are
  * not read), or dwg and dwu (then x is not).  Deterministic.  Takes 4*M*F bytes of
- * pool scratch (F rounded up to 8), plus copies and partial sums as above.  Without
- * rows dwg and dwu are zeros. */
+ * pool scratch (F rounded up to 8), plus copies and partial sums as above.  Gradients
+ * must not overlap the inputs or each other.  Without rows dwg and dwu are zeros. */
 BEE_B200_API int bee_b200_gated_linear_backward(int dt, int act, const void* x, size_t ldx, const void* wg,
                                                 const void* wu, size_t ldw, int trans, const void* g, const void* u,
                                                 const void* dout, void* dx, void* dwg, void* dwu, size_t lddw,

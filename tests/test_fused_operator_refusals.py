@@ -143,3 +143,16 @@ def test_gated_wrappers_refuse_what_is_no_matrix(monkeypatch):
             tc.gated_linear_backward(x, x, x, bad, x, x, dx=x)
     with pytest.raises(tc.BeeError):
         tc.gated_linear_backward(x, x, x, None, None, x, dx=x)
+
+
+@pytest.mark.parametrize("change", [{"out": P}, {"out": 2 * P}, {"out": 3 * P}, {"g": P, "u": 7 * P}, {"g": 6 * P, "u": 3 * P},
+                                    {"g": 6 * P, "u": 6 * P}, {"g": 4 * P, "u": 6 * P}])
+def test_gated_outputs_apart(change):
+    assert "overlap" in refused(*gated(**{"x": P, "wg": 2 * P, "wu": 3 * P, "out": 4 * P, **change}))
+
+
+@pytest.mark.parametrize("change", [{"dx": P}, {"dx": 2 * P}, {"dwg": 3 * P}, {"dwu": P}, {"dwg": 9 * P, "dwu": 9 * P},
+                                    {"dx": 9 * P, "dwg": 9 * P}])
+def test_gated_gradients_apart(change):
+    apart = {"x": P, "wg": 2 * P, "wu": 3 * P, "g": 4 * P, "u": 5 * P, "dout": 6 * P, "dx": 7 * P, "dwg": 8 * P, "dwu": 10 * P}
+    assert "overlap" in refused(*gated_backward(**{**apart, **change}))
