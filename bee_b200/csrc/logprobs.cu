@@ -27,7 +27,7 @@
 // elements that reach the bound than a list holds (many ties) insert them one by one into
 // sorted lists instead.
 // This costs latency at the end of a row (4 rows of 131072 bf16: 4.5 us without
-// alternatives, 8.6 us with 20); sorting the group maxima and merging the warps' lists
+// alternatives, 8.3 us with 20); sorting the group maxima and merging the warps' lists
 // took 1 to 4 us more, reading the whole shares of the threads concerned 2 to 10 us.
 //
 // Few rows: a cluster of up to 8 CTAs shares a row and joins its partial
