@@ -628,10 +628,12 @@ struct SumArgs {
     int ctas, items, by_border;
 };
 
-template <typename T, int SEGS> __global__ void __launch_bounds__(32 * SEGS) norm_residual_sum_kernel(const SumArgs a) {
-    __shared__ float4 part[SEGS][32];
-    const int lane = threadIdx.x & 31, seg = threadIdx.x >> 5;
-    const uint32_t col = blockIdx.x * 128 + lane * 4;
+// A block adds LANES * 4 columns: each LANES threads every SEGS-th partial row, then the warps' sums, in a fixed order.
+template <typename T, int LANES, int WARPS> __global__ void __launch_bounds__(32 * WARPS) norm_residual_sum_kernel(const SumArgs a) {
+    constexpr int SEGS = WARPS * 32 / LANES, COLS = LANES * 4;
+    __shared__ float4 part[WARPS][LANES];
+    const int lane = threadIdx.x % LANES, seg = threadIdx.x / LANES;
+    const uint32_t col = blockIdx.x * COLS + lane * 4;
     pdl_wait();
     for (int item = blockIdx.y; item < a.items; item += gridDim.y) {
         const float* src;
@@ -666,14 +668,21 @@ template <typename T, int SEGS> __global__ void __launch_bounds__(32 * SEGS) nor
                 s.w += v.w;
             }
         }
-        part[seg][lane] = s;
+#pragma unroll
+        for (int d = LANES; d < 32; d *= 2) {
+            s.x += __shfl_xor_sync(0xffffffffu, s.x, d);
+            s.y += __shfl_xor_sync(0xffffffffu, s.y, d);
+            s.z += __shfl_xor_sync(0xffffffffu, s.z, d);
+            s.w += __shfl_xor_sync(0xffffffffu, s.w, d);
+        }
+        if ((threadIdx.x & 31) < LANES) part[threadIdx.x >> 5][lane] = s;
         __syncthreads();
-        if (threadIdx.x < 128 && blockIdx.x * 128 + threadIdx.x < a.cols) {
+        if (threadIdx.x < COLS && blockIdx.x * COLS + threadIdx.x < a.cols) {
             const float* column = reinterpret_cast<const float*>(part) + threadIdx.x;
             float t = 0.f;
 #pragma unroll 8
-            for (int w = 0; w < SEGS; ++w) t += column[w * 128];
-            dst[blockIdx.x * 128 + threadIdx.x] = Conv<T>::down(t);
+            for (int w = 0; w < WARPS; ++w) t += column[w * COLS];
+            dst[blockIdx.x * COLS + threadIdx.x] = Conv<T>::down(t);
         }
         __syncthreads();
     }
@@ -753,10 +762,14 @@ template <typename T, bool VEC, int THREADS> int launch_bwd(NormArgs a, const No
         const int items = 2 + static_cast<int>(by_border ? borders : groups);
         const SumArgs s{a.part_post, a.part_pre, a.part_gate, g.dw_post, g.dw_pre, g.dgate, a.per_cta, a.group, a.cols, a.part,
                         static_cast<int>(ctas), items, by_border ? 1 : 0};
-        const dim3 grid((a.cols + 127) / 128, static_cast<unsigned>(items < 256 ? items : 256));
-        // a warp adds a few dozen rows at most: 586 partial rows took 37 us with 8 warps, 147 take 5 us
-        if (ctas > 256) launch_pdl(norm_residual_sum_kernel<T, 32>, grid, 1024, 0, st, s);
-        else launch_pdl(norm_residual_sum_kernel<T, 8>, grid, 256, 0, st, s);
+        // Many partial rows come with few columns: blocks of 32 columns (a 128-byte line of a row) spread them over
+        // the SMs (4099 x 1111 fp32, 684 partial rows: 35.7 us the whole call, 39.1 with 128 columns and 32 warps;
+        // 65536 x 512 bf16 76.1 against 80.8).  The gate groups that CTAs cut are many items of a few partial rows,
+        // for which wide blocks are faster (20000 x 1500 fp32, groups of 10: 186 us against 198).
+        const dim3 wide((a.cols + 127) / 128, static_cast<unsigned>(items < 256 ? items : 256));
+        if (ctas <= 256) launch_pdl(norm_residual_sum_kernel<T, 32, 8>, wide, 256, 0, st, s);
+        else if (items > 8) launch_pdl(norm_residual_sum_kernel<T, 32, 32>, wide, 1024, 0, st, s);
+        else launch_pdl(norm_residual_sum_kernel<T, 8, 16>, dim3((a.cols + 31) / 32, static_cast<unsigned>(items)), 512, 0, st, s);
         rc = launch_status("norm_gate_residual_backward (sums)");
     }
     const cudaError_t e2 = cudaFreeAsync(mem, st);
