@@ -273,8 +273,10 @@ __device__ __forceinline__ long long target_of(const void* t, int is64, long lon
 }
 
 constexpr int kUnroll = 4;  // chunks of a thread per batch
-constexpr int kMaxCluster = 8;
 constexpr int kStages = 3;  // batches in its part of the shared-memory ring
+// CTAs that may share a row.  A row of a 128-thread block has at most 513 chunks, for which cluster_for never
+// gains from more than 4.
+constexpr int max_cluster(int threads) { return threads == 128 ? 4 : 8; }
 
 // 16 bytes from global to shared memory, both addresses moved by OFF bytes.
 template <int OFF> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -301,6 +303,22 @@ template <typename T> struct Part {
     }
 };
 
+// A forward CTA's shared memory beside its ring.
+template <int THREADS, bool TOP> struct ForwardShared {
+    static constexpr int WARPS = THREADS / 32, CLUSTER = max_cluster(THREADS);
+    Stat warp_stat[WARPS];
+    Stat cta_stat[CLUSTER];  // rank 0's copy is filled by the whole cluster
+    // for the alternatives:
+    alignas(16) float group_max[TOP ? 64 : 4];
+    float lane_max[TOP ? WARPS : 1][32];
+    uint64_t lists[TOP ? WARPS : 1][32];  // each warp's elements that reach the bound
+    uint64_t sorted[TOP ? 32 : 1];
+    uint64_t cta_list[TOP ? CLUSTER : 1][32];
+    int listed[WARPS];
+
+    static constexpr int RING = sizeof(uint4) * kStages * kUnroll * THREADS;
+};
+
 // Clusters of `cluster` CTAs (1: single CTAs) take rows in grid-stride order.
 // Every thread streams its own chunks of the coming batches, across rows, into
 // its own slots of a ring with cp.async, so that loads stay in flight while a row
@@ -309,16 +327,20 @@ template <typename T, int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const LogprobArgs a, int cluster) {
     constexpr int WARPS = THREADS / 32;
     constexpr int E = Elems<T>::E;
-    extern __shared__ __align__(16) uint4 ring[];  // [kStages][kUnroll][THREADS]; four CTAs of 256 threads leave 8 KiB each for the rest
-    __shared__ Stat warp_stat[WARPS];
-    __shared__ Stat cta_stat[kMaxCluster];  // rank 0's copy is filled by the whole cluster
-    // 7.5 KiB for the alternatives: four CTAs of 256 threads and their rings fill an SM's shared memory
-    __shared__ uint64_t lists[TOP ? WARPS : 1][32];  // each warp's elements that reach the bound
-    __shared__ int listed[WARPS];
-    __shared__ uint64_t sorted[TOP ? 32 : 1];
-    __shared__ uint64_t cta_list[TOP ? kMaxCluster : 1][32];
-    __shared__ __align__(16) float group_max[TOP ? 64 : 4];
-    __shared__ float lane_max[TOP ? WARPS : 1][32];
+    using Shared = ForwardShared<THREADS, TOP>;
+    // The grid is made for 1024 threads per SM: a CTA that found no place would wait for all the rows of another.  (An
+    // SM has 228 KiB, and each CTA takes 1 KiB beside its own.)
+    static_assert((sizeof(Shared) + Shared::RING + 1024) * (1024 / THREADS) <= 228 * 1024, "fewer CTAs fit an SM than the grid is made for");
+    extern __shared__ __align__(16) uint4 ring[];  // [kStages][kUnroll][THREADS]
+    __shared__ Shared sh;
+    auto& warp_stat = sh.warp_stat;
+    auto& cta_stat = sh.cta_stat;
+    auto& group_max = sh.group_max;
+    auto& lane_max = sh.lane_max;
+    auto& lists = sh.lists;
+    auto& cta_list = sh.cta_list;
+    auto& sorted = sh.sorted;
+    auto& listed = sh.listed;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = cluster > 1 ? static_cast<int>(sm100::cluster_ctarank()) : 0;
     const float c = a.inv_t * kLog2e;
@@ -786,10 +808,10 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS) token_logprobs_grad_k
 // CTAs that share a row: the cluster size with the least work on the slowest
 // CTA, a row costing its share of the chunks plus about 1024 chunks' time for its
 // joins, and 128 more for each doubling of the cluster.
-int cluster_for(long long rows, long long chunks, long long slots) {
+int cluster_for(long long rows, long long chunks, long long slots, int most) {
     int best = 1;
     double least = 0, joins = 1024;
-    for (int cl = 1; cl <= kMaxCluster; cl *= 2, joins += 128) {
+    for (int cl = 1; cl <= most; cl *= 2, joins += 128) {
         const long long clusters = slots / cl;
         const double cost = static_cast<double>((rows + clusters - 1) / clusters) * (static_cast<double>(chunks) / cl + joins);
         if (cl == 1 || cost < least) {
@@ -803,8 +825,8 @@ int cluster_for(long long rows, long long chunks, long long slots) {
 template <typename T, int THREADS, bool TOP> int launch_forward(const LogprobArgs& a, cudaStream_t st) {
     const long long chunks = (a.vocab + Elems<T>::E - 1) / Elems<T>::E + 1;
     const long long slots = static_cast<long long>(sm_count()) * (1024 / THREADS);
-    const int cl = cluster_for(a.rows, chunks, slots);
-    const size_t smem = sizeof(uint4) * kStages * kUnroll * THREADS;
+    const int cl = cluster_for(a.rows, chunks, slots, max_cluster(THREADS));
+    const size_t smem = ForwardShared<THREADS, TOP>::RING;
     auto logprobs_kern = token_logprobs_kernel<T, THREADS, TOP>;
     static SmemLimit limit;
     if (int rc = limit.ensure(logprobs_kern, static_cast<int>(smem), "token_logprobs")) return rc;
