@@ -54,15 +54,18 @@ __device__ __forceinline__ float activation(float g, int act) {
     return g * sigmoid(2.f * kTanhC * fmaf(kTanhA * g * g, g, g));
 }
 
-// The activation and its derivative.  Past |g| = 32 every derivative is 0 or 1
-// to the last bit; clamping there keeps the products below from overflowing.
+// The activation and its derivative.  The factors of p = sigmoid or Phi that grow with g take a clamped g, so that
+// they stay finite where p is 0 or 1 to the last bit and the derivative with it: past |g| = 88 for silu, whose p is
+// still e^g below it, and past 32 for the gelus.
 __device__ __forceinline__ void activation_grad(float g, int act, float& a, float& da) {
-    const float c = fminf(fmaxf(g, -32.f), 32.f);
     if (act == ACT_SILU) {
         const float p = sigmoid(g);
         a = g * p;
-        da = p * fmaf(c, 1.f - p, 1.f);
-    } else if (act == ACT_GELU) {
+        da = p * fmaf(fminf(fmaxf(g, -128.f), 128.f), 1.f - p, 1.f);
+        return;
+    }
+    const float c = fminf(fmaxf(g, -32.f), 32.f);
+    if (act == ACT_GELU) {
         const float p = normcdff(g);
         a = g * p;
         da = fmaf(c * 0.3989422804014327f, exp2f(-0.5f * kLog2e * c * c), p);
