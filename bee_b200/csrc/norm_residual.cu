@@ -803,6 +803,17 @@ int check(const char* what, int dt, size_t rows, size_t cols, size_t group, bool
     return 0;
 }
 
+// A tensor's bytes; an absent one has none.
+struct Span {
+    const void* p;
+    size_t bytes;
+    bool meets(const Span& o) const {
+        const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(o.p);
+        return p && o.p && a < b + o.bytes && b < a + bytes;
+    }
+    bool crosses(const Span& o) const { return p != o.p && meets(o); }  // overlaps, and is not the same tensor
+};
+
 // Every given pointer is aligned to `to` bytes.
 template <typename... P> bool aligned(uintptr_t to, const P*... p) { return (((reinterpret_cast<uintptr_t>(p)) | ...) & (to - 1)) == 0; }
 
@@ -824,6 +835,16 @@ int bee_b200_norm_gate_residual(int dt, const void* h, const void* x, const void
     const size_t elem = dt == DT_F32 ? 4 : 2;
     if (!aligned(elem, h, x, w_post, gate, w_pre, x_out, y))
         return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    // rows are read ahead and by many CTAs: an output may take the place of h or x only row by row
+    const size_t vector = cols * elem, tensor = rows * vector;
+    const Span in[2] = {{h, tensor}, {x, tensor}}, out[2] = {{x_out, tensor}, {w_pre ? y : nullptr, tensor}};
+    const Span vectors[3] = {{w_post, vector}, {gate, group ? rows / group * vector : vector}, {w_pre, vector}};
+    bool apart = !out[0].meets(out[1]);
+    for (const Span& o : out) {
+        for (const Span& i : in) apart = apart && !o.crosses(i);
+        for (const Span& v : vectors) apart = apart && !o.meets(v);
+    }
+    if (!apart) return fail(cudaErrorInvalidValue, "%s: outputs must not overlap each other, nor an input unless x_out or y is h or x", what);
     NormArgs a{};
     a.h = h; a.x = x; a.w_post = w_post; a.gate = gate; a.w_pre = w_pre; a.x_out = x_out; a.y = y;
     a.rows = static_cast<long long>(rows);
@@ -856,6 +877,22 @@ int bee_b200_norm_gate_residual_backward(int dt, const void* h, const void* x, c
     if (!h || !x || !dh || !dx || (w_pre && !dy) || (!dx_out && !w_pre)) return fail(cudaErrorInvalidValue, "%s: null pointer", what);
     if (!aligned(elem, h, x, w_post, gate, w_pre, dx_out, dy, dh, dx, dw_post, dgate, dw_pre))
         return fail(cudaErrorInvalidValue, "%s: a tensor is not aligned to its type", what);
+    // as in the forward; gate gradients are written while other rows are read, those of the weights after all of them
+    const size_t vector = cols * elem, tensor = rows * vector, gates = group ? rows / group * vector : vector;
+    const Span in[4] = {{h, tensor}, {x, tensor}, {dx_out, tensor}, {w_pre ? dy : nullptr, tensor}};
+    const Span vectors[3] = {{w_post, vector}, {gate, gates}, {w_pre, vector}};
+    const Span out[5] = {{dh, tensor}, {dx, tensor}, {gate ? dgate : nullptr, gates}, {w_post ? dw_post : nullptr, vector},
+                         {w_pre ? dw_pre : nullptr, vector}};
+    bool apart = true;
+    for (int i = 0; i < 5; ++i)
+        for (int j = 0; j < i; ++j) apart = apart && !out[i].meets(out[j]);
+    for (int o = 0; o < 2; ++o) {
+        for (const Span& i : in) apart = apart && !out[o].crosses(i);
+        for (const Span& v : vectors) apart = apart && !out[o].meets(v);
+    }
+    for (const Span& i : in) apart = apart && !out[2].meets(i);
+    apart = apart && !out[2].meets(vectors[0]) && !out[2].meets(vectors[2]) && !out[2].crosses(vectors[1]);
+    if (!apart) return fail(cudaErrorInvalidValue, "%s: gradients must not overlap each other, nor an input unless dh or dx is one of its shape", what);
     NormArgs a{};
     a.h = h; a.x = x; a.w_post = w_post; a.gate = gate; a.w_pre = w_pre;
     a.dx_out = dx_out; a.dy = w_pre ? dy : nullptr; a.dh = dh; a.dx = dx; a.dgate = dgate;

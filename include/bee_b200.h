@@ -222,7 +222,8 @@ BEE_B200_API int bee_b200_rms_norm_rows(int dt, const void* x, const void* w, vo
  * [rows / group, cols], one for each `group` consecutive rows (e.g. a sequence).
  * One dtype for all tensors, in {F32, BF16, F16}; math in fp32 with one rounding
  * per output (y from the unrounded x_out); contiguous tensors, cols <= 16384
- * (F32: 12288).  x_out may be x or h, y may be h or x (not both the same one).
+ * (F32: 12288).  x_out and y may each be h or x (not both the same one);
+ * beyond that an output that overlaps an input or the other output is refused.
  * Fastest when cols is a whole number of 16-byte vectors and all tensors are
  * 16-byte aligned. */
 BEE_B200_API int bee_b200_norm_gate_residual(int dt, const void* h, const void* x, const void* w_post, const void* gate,
@@ -236,7 +237,8 @@ BEE_B200_API int bee_b200_norm_gate_residual(int dt, const void* h, const void* 
  * (fp32 sums over the rows, rounded once).  Deterministic.  The partial sums take
  * 16 bytes per column and CTA (at most 16 CTAs per SM) of the stream-ordered pool,
  * returned on the stream.  dh and dx may each be any one of the inputs of their
- * shape.  Without rows the gradients of the vectors are zeros. */
+ * shape (not both the same one); gradients that overlap each other, or dh, dx or
+ * dgate any other input, are refused.  Without rows the gradients of the vectors are zeros. */
 BEE_B200_API int bee_b200_norm_gate_residual_backward(int dt, const void* h, const void* x, const void* w_post,
                                                       const void* gate, const void* w_pre, const void* dx_out,
                                                       const void* dy, void* dh, void* dx, void* dw_post, void* dgate,
