@@ -739,7 +739,8 @@ __device__ __forceinline__ RowGrad row_grad(const LogprobGradArgs& a, long long 
     RowGrad g;
     const float m = a.row_max[r];
     g.target = a.dlogprob ? target_of(a.targets, a.targets_i64, r) : -1;
-    const float gl = g.target >= 0 ? a.dlogprob[r] : 0.f;
+    float gl = g.target >= 0 ? a.dlogprob[r] : 0.f;
+    if (g.target >= a.vocab && gl != 0.f) gl = NAN;  // as the forward's logprob
     const float gh = a.dentropy ? a.dentropy[r] : 0.f;
     g.m = m;
     g.c = a.inv_t * kLog2e;

@@ -284,9 +284,10 @@ BEE_B200_API int bee_b200_token_logprobs(int dt, const void* logits, size_t ld, 
  *   dlogits_i = (dlogprob (delta_{i,target} - p_i) - dentropy p_i (logp_i + entropy)) / temperature
  * in the logits' dtype (row stride ldd).  row_max, log_sum and (when dentropy is
  * given) entropy are the forward's outputs; dlogprob (with targets) and dentropy
- * may each be NULL.  Rows without a token take no gradient from dlogprob; rows
- * whose gradients are both 0, and rows with every logit masked, get zeros
- * whatever they hold.  dlogits may be the logits themselves (same stride). */
+ * may each be NULL.  Rows without a token take no gradient from dlogprob; a target
+ * >= vocab whose dlogprob is not 0 gives NaN, as its logprob is; rows whose
+ * gradients are both 0, and rows with every logit masked, get zeros whatever they
+ * hold.  dlogits may be the logits themselves (same stride). */
 BEE_B200_API int bee_b200_token_logprobs_backward(int dt, const void* logits, size_t ld, int targets_dt,
                                                   const void* targets, size_t rows, size_t vocab, float temperature,
                                                   const float* row_max, const float* log_sum, const float* entropy,
