@@ -82,10 +82,10 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most `pending` (0 or 1: a ring has up to three slots) of the thread's groups are in flight.
 __device__ __forceinline__ void cp_wait(int pending) {
     if (pending == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-    else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 1;" ::: "memory");
 }
 
 // The columns of one thread.  VEC: 16-byte vectors tid, tid + THREADS, ...;
@@ -231,15 +231,15 @@ template <typename T, bool VEC, int THREADS> struct Cols {
     }
 };
 
-// Sums over the block with one barrier: consecutive calls use alternating halves
+// Two sums over the block with one barrier: consecutive calls use alternating rows
 // of `red`, so a call's writes never meet the previous call's reads.
 template <int THREADS> struct BlockSum {
     static constexpr int WARPS = (THREADS / 32 + 3) / 4 * 4;  // those past the block's add 0
-    f2 (*red)[WARPS];  // rows 0 and 1: a warp's two sums; rows 2 and 3, as floats: its only one
+    f2 (*red)[WARPS];  // two rows of the warps' two sums
     int parity = 0;
     __device__ __forceinline__ explicit BlockSum(f2 (*r)[WARPS]) : red(r) {
         if constexpr (THREADS / 32 < WARPS) {
-            for (int i = threadIdx.x; i < 4 * WARPS; i += THREADS) r[i / WARPS][i % WARPS] = 0;
+            for (int i = threadIdx.x; i < 2 * WARPS; i += THREADS) r[i / WARPS][i % WARPS] = 0;
             __syncthreads();
         }
     }
@@ -260,21 +260,6 @@ template <int THREADS> struct BlockSum {
         float2 s;
         unpack_f32x2(r, s.x, s.y);
         return s;
-    }
-    __device__ __forceinline__ float operator()(float a) {
-        a = warp_sum(a);
-        if constexpr (THREADS == 32) return a;
-        float* one = reinterpret_cast<float*>(red[2 + parity]);
-        if ((threadIdx.x & 31) == 0) one[threadIdx.x >> 5] = a;
-        __syncthreads();
-        f2 r = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; w += 4) {
-            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(one + w);
-            r = add_f32x2(add_f32x2(r, v.x), v.y);
-        }
-        parity ^= 1;
-        return hsum(r);
     }
 };
 
@@ -371,7 +356,7 @@ struct NormArgs {
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
+    __shared__ __align__(16) f2 red[2][BlockSum<THREADS>::WARPS];
     BlockSum<THREADS> block_sum(red);
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
@@ -453,7 +438,7 @@ template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) norm_residual_grad_kernel(const NormArgs a) {
     constexpr bool KEEP = keep_vectors<T>(THREADS);
     extern __shared__ __align__(16) uint8_t ring_smem[];
-    __shared__ __align__(16) f2 red[4][BlockSum<THREADS>::WARPS];
+    __shared__ __align__(16) f2 red[2][BlockSum<THREADS>::WARPS];
     BlockSum<THREADS> block_sum(red);
     const Cols<T, VEC, THREADS> cl(a.cols);
     const long long r0 = blockIdx.x * a.per_cta;
@@ -618,8 +603,7 @@ __global__ void __launch_bounds__(THREADS, THREADS <= 512 ? 512 / THREADS : 1) n
 // Adds the CTAs' partial sums.  Item 0 is w_post, 1 is w_pre, the others are gate
 // groups: 2 + g is group g (by_border == 0), or 1 + c the group that the border
 // between CTAs c - 1 and c is the first to cut, if there is one, so that there are at
-// most as many items as groups and as borders.  A block takes 128 columns, four per
-// lane; its SEGS warps add every SEGS-th CTA's row and are joined in order.
+// most as many items as groups and as borders.
 struct SumArgs {
     const float *part_post, *part_pre, *part_gate;
     void *dw_post, *dw_pre, *dgate;
