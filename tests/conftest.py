@@ -19,6 +19,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a B200 GPU; runs the CUDA kernels through the C ABI")
 
 
+def pytest_collection_modifyitems(items):
+    """The drop-in Tensor library is built from the reference's sources (make -C oracle tensor-cuda).  Where it has not
+    been built its GPU test fails and says so; it goes last, so that a run that ends at the first failure (-x) has run
+    everything else."""
+    if not (ROOT / "oracle" / "_ref" / "test_bee_tensor_cuda").exists():
+        items.sort(key=lambda item: item.path.name == "test_gpu_bee_tensor.py")
+
+
 @pytest.fixture(scope="session")
 def oracle():
     from oracle.oracle import Oracle
