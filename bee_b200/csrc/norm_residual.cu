@@ -352,7 +352,7 @@ struct NormArgs {
 // ---------------------------------------------------------------- forward
 
 // The vectors come from L1 for every row: holding beta gate w_post and w_pre in
-// registers leaves three quarters of the threads (32768 x 4096 bf16: 190 us, 179 so).
+// registers leaves three quarters of the threads (32768 x 4096 bf16, cold caches: 191 us, 186 so).
 template <typename T, bool VEC, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) norm_residual_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t ring_smem[];
@@ -697,6 +697,9 @@ template <typename T, bool VEC, int THREADS> int launch_fwd(NormArgs a, cudaStre
     return launch_status("norm_gate_residual");
 }
 
+// The block with the fewest idle columns.  Without the blocks of 160 and 384 threads (bf16, cold caches, forward /
+// backward): 16384 x 2560 79.9 / 131.7 us in 256 threads, 65.5 / 96.9 in 160; 8192 x 6144 84.0 / 148.1 us in 512,
+// 77.8 / 127.6 in 384 (fp32 there 139.3 / 252.5 and 135.2 / 254.6).
 template <typename T, bool VEC> int forward(const NormArgs& a, cudaStream_t st) {
     if (a.cols <= 32 * kEpt) return launch_fwd<T, VEC, 32>(a, st);
     if (a.cols <= 64 * kEpt) return launch_fwd<T, VEC, 64>(a, st);

@@ -362,7 +362,8 @@ BEE_B200_API int bee_b200_gated_linear(int dt, int act, const void* x, size_t ld
                                        size_t F, bee_b200_stream_t stream);
 
 /* Its gradient, from x, the weights, the forward's g and u and dout (g, u, dout
- * [M, F] contiguous):  dg = dout u act'(g) and du = dout act(g), rounded to dt;
+ * [M, F] contiguous):  dg = dout u act'(g) and du = dout act(g), rounded to dt
+ * (the tensor cores' operand type; an F16 one past 65504 becomes inf);
  * dx = dg Wg^T + du Wu^T [M, D] contiguous; dwg = x^T dg and dwu = x^T du in the
  * weights' layout with row stride lddw.  dx may be NULL (then the weights are
  * not read), or dwg and dwu (then x is not).  Deterministic.  Takes 4*M*F bytes of
