@@ -206,8 +206,8 @@ struct PairCfg {
 };
 
 // One epilogue warp's 32 rows x 64 columns: rounded into its next staging buffer (128-byte rows, swizzled as the map
-// says) and stored by TMA, which cuts what lies outside the output; outputs that TMA cannot describe (odd strides) are
-// written from the buffer row by row, a column per lane.  v(j): the lane's row's column j.
+// says) and stored by TMA, which cuts what lies outside the output in whole 16-byte blocks only; outputs whose strides
+// or columns are no whole number of those are written from the buffer row by row, a column per lane.  v(j): the lane's row's column j.
 template <typename V>
 __device__ __forceinline__ void store_block(const PairParams& p, const CUtensorMap* map, uint16_t* out, uint8_t* stage, int& turn, int lane,
                                             int row0, int col, V v) {
@@ -1064,7 +1064,7 @@ int bee_b200_gated_linear_backward(int dt, int act, const void* x, size_t ldx, c
         p.ldc = static_cast<long long>(lddw);
         p.out[0] = static_cast<uint16_t*>(dwg);
         p.out[1] = static_cast<uint16_t*>(dwu);
-        p.vec = lddw % 8 == 0 && aligned16(dwg) && aligned16(dwu);
+        p.vec = lddw % 8 == 0 && wcols % 8 == 0 && aligned16(dwg) && aligned16(dwu);  // else what follows a row would be written
         p.f16 = f16;
         p.a_second = trans ? 1 : 0;
         if (rc == 0) rc = trans ? launch_pair<DW, true, true>(dg, du, mx, mx, p, what, st) : launch_pair<DW, true, true>(mx, mx, dg, du, p, what, st);
