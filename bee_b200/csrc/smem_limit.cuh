@@ -20,7 +20,7 @@ int api_fail(cudaError_t e, const char* fmt, ...);
 // function-local static.
 constexpr int kMaxDevices = 64;
 struct SmemLimit {
-    std::atomic<int> raised[kMaxDevices];
+    std::atomic<int> raised[kMaxDevices]{};
     std::mutex raising;
     template <typename Kernel>
     int ensure(Kernel kernel, int bytes, const char* what) {
