@@ -68,11 +68,17 @@ cudaError_t pool_malloc(void** ptr, size_t bytes, cudaStream_t st) {
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!pools[dev]) {
-            cudaMemPool_t p = nullptr;
-            e = cudaDeviceGetDefaultMemPool(&p, dev);
+            // A first call may be one that is being captured: setting the pool up is no part of that graph, and in the
+            // stricter capture modes it would end the capture.
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            e = cudaThreadExchangeStreamCaptureMode(&mode);
             if (e != cudaSuccess) return e;
+            cudaMemPool_t p = nullptr;
             uint64_t keep = ~uint64_t{0};
-            e = cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep);
+            e = cudaDeviceGetDefaultMemPool(&p, dev);
+            if (e == cudaSuccess) e = cudaMemPoolSetAttribute(p, cudaMemPoolAttrReleaseThreshold, &keep);
+            const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+            if (e == cudaSuccess) e = back;
             if (e != cudaSuccess) return e;
             pools[dev] = p;
         }
